@@ -468,6 +468,58 @@ int  azg_train_loss_bwd(const float* x3, int32_t ld3, const float* z4, int32_t l
                         const float* tv, const float* rows, int32_t B, int32_t A, const float* g, float* dx3,
                         int32_t lddx, float* dz4, int32_t lddz, void* stream);
 
+/* ---- operators over rows of policy logits (azg_policy.hip; azg_amd.policy) ---------------------------
+ * azg_logits: `rows` rows of `vocab` logits (f32, bf16 or f16), row r at element offset
+ *   (r / inner) * stride_outer + (r % inner) * stride_inner of x (>= 0; rows may overlap or repeat), its
+ *   elements adjacent; mask: null, or one byte per action (0: illegal) at the mask's own two strides
+ *   (0 repeats one mask); every probability below is over the legal actions, of logits / temperature.
+ * azg_teacher: per row k entries (id, log-probability), contiguous [rows][k]; an id outside
+ *   [0, vocab) or a log-probability of -inf is no entry.  rest = 0: the entries' probabilities are
+ *   softmax(logp); rest = 1: exp(logp), and what they leave of one is the mass of all other actions.
+ * azg_logprobs_fwd: logp [rows] of actions [rows] (both null: none; int64 when actions64, else int32; an
+ *   action outside [0, vocab): 0, an illegal one: -inf), entropy [rows], lse [rows] = ln sum exp, and the
+ *   `top` largest legal logits of each row as top_logp / top_ids [rows][top] (ties: lower index first;
+ *   fewer than top: -inf / -1).  stats [rows][4] (16-B aligned, may be null) is what the backward needs.
+ *   A row without a legal action: entropy 0, lse and logp -inf, ids -1.
+ * azg_logprobs_bwd: dx [rows][vocab] (contiguous, logits' type) from the gradients of logp / entropy / lse
+ *   (each may be null; element r at r * its stride, 0 repeats one value); 0 at illegal actions.
+ * azg_distill_fwd: row_loss [rows] = KL(teacher || student), 0 for a row without an entry or without a
+ *   legal action; total (may be null) = scale sum_r weight_r row_loss_r (weight null: 1; a stride of 0
+ *   repeats one value; f64, fixed order); dx (may be null) = the gradient of that sum.  stats [rows][8]
+ *   (16-B aligned, may be null without dx) is what azg_distill_bwd needs, which writes dx = the gradient of
+ *   scale sum_r weight_r row_loss_r.
+ * work: azg_logprobs_work / azg_distill_work bytes of scratch (16-B aligned; 0: may be null; -1: a bad
+ *   argument), in use until the call's kernels end.  1 <= rows <= AZG_POLICY_ROWS_MAX, 1 <= vocab <= AZG_POLICY_VOCAB_MAX. */
+#define AZG_POLICY_TOP_MAX 128
+#define AZG_POLICY_ROWS_MAX (1LL << 35)
+#define AZG_POLICY_VOCAB_MAX (1LL << 30)
+enum azg_dtype { AZG_F32 = 0, AZG_BF16 = 1, AZG_F16 = 2 };
+typedef struct azg_logits {
+    const void* x;
+    const uint8_t* mask;
+    int64_t rows, inner, stride_outer, stride_inner, mask_outer, mask_inner, vocab;
+    int32_t dtype;
+    float temperature;
+} azg_logits;
+typedef struct azg_teacher {
+    const void* logp;
+    const void* ids;
+    int32_t dtype, ids64, k, rest;
+} azg_teacher;
+int64_t azg_logprobs_work(const azg_logits* L, int32_t top);
+int64_t azg_distill_work(const azg_logits* L, int32_t grad);
+int  azg_logprobs_fwd(const azg_logits* L, const void* actions, int32_t actions64, int32_t top, float* stats,
+                      float* logp, float* entropy, float* lse, float* top_logp, int64_t* top_ids, void* work,
+                      int64_t work_bytes, void* stream);
+int  azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_t actions64, const float* stats,
+                      const float* g_logp, int64_t g_logp_stride, const float* g_entropy, int64_t g_entropy_stride,
+                      const float* g_lse, int64_t g_lse_stride, void* dx, void* stream);
+int  azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float* stats, float* row_loss, const float* weight,
+                     int64_t weight_stride, float scale, float* total, void* dx, void* work, int64_t work_bytes,
+                     void* stream);
+int  azg_distill_bwd(const azg_logits* L, const azg_teacher* t, const float* stats, const float* weight,
+                     int64_t weight_stride, float scale, void* dx, void* stream);
+
 /* ---- the trainer's optimizer (azg_adam.hip) -------------------------------------------------
  * azg_adam_step: torch.optim.Adam's step (NNet.py:37; the capturable foreach arithmetic of
  * torch/optim/adam.py in f32, no weight decay / amsgrad) over nseg parameter tensors in one launch:
