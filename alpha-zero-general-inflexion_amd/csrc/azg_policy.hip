@@ -18,6 +18,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "../../include/azg.h"
 
@@ -28,6 +29,8 @@ namespace {
 constexpr int TOP_MAX = AZG_POLICY_TOP_MAX;
 constexpr float LN2 = 0.69314718055994530942f;
 constexpr float LOWEST = -3.402823466e38f;
+constexpr float FAR = 1.2676506e30f;  // 2^100: beyond any log2 of a ratio that a sum can hold
+constexpr int GROUP = 4;              // 16-byte loads that a thread has in flight together
 
 using bf16_t = __bf16;
 using f16_t = _Float16;
@@ -59,21 +62,242 @@ dim3 row_grid(long long rows) {
     return dim3((unsigned)x, (unsigned)((rows + x - 1) / x));
 }
 
-// max that keeps a NaN (fmaxf drops it): a NaN logit makes its row's statistics NaN
+
+// max that keeps a NaN (fmaxf drops it, and costs a canonicalisation of what was loaded)
 __device__ __forceinline__ float nmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = nmax(x, __shfl_xor(x, o));
-    return x;
+// ---- wave and team reductions -------------------------------------------------------------------
+// Within rows of 16 lanes by DPP (the partner's value arrives with the instruction, no LDS round trip), the four
+// rows by readlane.  Every lane gets the result; the order is fixed.
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned x) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
 }
-template <class F>
-__device__ __forceinline__ F wave_sum(F x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) { return __uint_as_float(dpp<CTRL>(__float_as_uint(x))); }
+template <int CTRL>
+__device__ __forceinline__ unsigned long long dpp(unsigned long long x) {
+    return ((unsigned long long)dpp<CTRL>((unsigned)(x >> 32)) << 32) | dpp<CTRL>((unsigned)x);
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    return __longlong_as_double((long long)dpp<CTRL>((unsigned long long)__double_as_longlong(x)));
+}
+__device__ __forceinline__ unsigned lane_of(unsigned x, int l) { return (unsigned)__builtin_amdgcn_readlane((int)x, l); }
+__device__ __forceinline__ float lane_of(float x, int l) { return __uint_as_float(lane_of(__float_as_uint(x), l)); }
+__device__ __forceinline__ unsigned long long lane_of(unsigned long long x, int l) {
+    return ((unsigned long long)lane_of((unsigned)(x >> 32), l) << 32) | lane_of((unsigned)x, l);
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+    return __longlong_as_double((long long)lane_of((unsigned long long)__double_as_longlong(x), l));
+}
+constexpr int QUAD_XOR1 = 0xB1, QUAD_XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
+template <class V, class F>
+__device__ __forceinline__ V wave_reduce(V x, F f) {
+    x = f(x, dpp<QUAD_XOR1>(x));
+    x = f(x, dpp<QUAD_XOR2>(x));
+    x = f(x, dpp<HALF_MIRROR>(x));
+    x = f(x, dpp<MIRROR>(x));
+    return f(f(lane_of(x, 0), lane_of(x, 16)), f(lane_of(x, 32), lane_of(x, 48)));
+}
+template <class V>
+__device__ __forceinline__ V wave_sum(V x) { return wave_reduce(x, [](V a, V b) { return a + b; }); }
+__device__ __forceinline__ float wave_max(float x) { return wave_reduce(x, [](float a, float b) { return nmax(a, b); }); }
+
+// A team is the threads that share a row: a wave (64; four teams in a block) or a block.
+template <int TEAM>
+__device__ __forceinline__ void team_sync() {
+    if constexpr (TEAM == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // the wave's own LDS and global accesses, in order
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+template <int TEAM>
+constexpr int block_of = TEAM == 64 ? 256 : TEAM;
+template <int TEAM>
+__device__ __forceinline__ int team_tid() { return TEAM == 64 ? threadIdx.x & 63 : threadIdx.x; }
+template <int TEAM>
+__device__ __forceinline__ int team_in_block() { return TEAM == 64 ? threadIdx.x >> 6 : 0; }
+template <int TEAM>
+__device__ __forceinline__ long long team_row() { return TEAM == 64 ? block_row() * 4 + (threadIdx.x >> 6) : block_row(); }
+
+// ---- vectors of 16 bytes (a row may start at any element: the loads need no more than its alignment) ----
+template <class T>
+constexpr int VN = 16 / (int)sizeof(T);
+template <class T>
+constexpr unsigned MINF_BITS = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, f16_t> ? 0xFC00FC00u : 0xFF80FF80u;
+
+template <class T>
+__device__ __forceinline__ uint4 load16(const T* p) {
+    uint4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& v, float* f) {
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, bf16_t>) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            f[2 * i] = (float)__builtin_bit_cast(f16_t, (unsigned short)w[i]);
+            f[2 * i + 1] = (float)__builtin_bit_cast(f16_t, (unsigned short)(w[i] >> 16));
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void store16(T* p, const float* f) {
+    T t[VN<T>];
+#pragma unroll
+    for (int i = 0; i < VN<T>; ++i) t[i] = (T)f[i];  // round to nearest even
+    __builtin_memcpy(p, t, 16);
+}
+// illegal actions of a vector -> -inf
+template <class T>
+__device__ __forceinline__ void apply_mask(const uint8_t* mk, float* f) {
+    uint8_t b[VN<T>];
+    __builtin_memcpy(b, mk, VN<T>);
+#pragma unroll
+    for (int i = 0; i < VN<T>; ++i) f[i] = b[i] ? f[i] : -INFINITY;
+}
+
+// ---- softmax statistics -------------------------------------------------------------------------
+// s = sum 2^u, w = sum u 2^u with u = x c - r and r a whole number near max x c: moving a sum to another r is exact
+// (a power of two), and x c - r is one rounding.  r follows the maximum lazily (u <= 8.5), and starts at -2^100 with
+// an empty sum.  Where |x c| passes 2^100 (the type's lowest value in f32 and bf16) or a logit is no number, the row
+// is done again by `Soft` below, with u = (x - m) c.
+struct Sum {
+    float r, s, w;
+};
+template <bool ENT, int N>
+__device__ __forceinline__ void sum_group(Sum& a, const float* x, float gm, float c) {
+    if (__builtin_fmaf(gm, c, -a.r) > 8.f) {
+        const float r = rintf(gm * c), d = a.r - r;
+        if constexpr (ENT) a.w = __builtin_amdgcn_ldexpf(__builtin_fmaf(d, a.s, a.w), (int)fmaxf(d, -4096.f));
+        a.s = __builtin_amdgcn_ldexpf(a.s, (int)fmaxf(d, -4096.f));
+        a.r = r;
+    }
+    float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float u0 = __builtin_fmaf(x[i], c, -a.r), u1 = __builtin_fmaf(x[i + 1], c, -a.r);
+        const float e0 = ex2(u0), e1 = ex2(u1);
+        s0 += e0;
+        s1 += e1;
+        if constexpr (ENT) {
+            w0 = __builtin_fmaf(e0, nmax(u0, -1000.f), w0);
+            w1 = __builtin_fmaf(e1, nmax(u1, -1000.f), w1);
+        }
+    }
+    a.s += s0 + s1;
+    if constexpr (ENT) a.w += w0 + w1;
+}
+__device__ __forceinline__ Sum move_sum(Sum a, float r) {  // to a reference r >= a.r
+    const float d = a.r - r;
+    const int k = (int)fmaxf(d, -4096.f);
+    return Sum{r, __builtin_amdgcn_ldexpf(a.s, k), __builtin_amdgcn_ldexpf(__builtin_fmaf(d, a.s, a.w), k)};
+}
+template <int TEAM>
+__device__ __forceinline__ Sum team_sum(Sum a, Sum* sh) {
+    a = move_sum(a, wave_max(a.r));
+    a.s = wave_sum(a.s);
+    a.w = wave_sum(a.w);
+    if constexpr (TEAM > 64) {
+        constexpr int W = TEAM / 64;
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+        __syncthreads();
+        float r = sh[0].r;
+#pragma unroll
+        for (int i = 1; i < W; ++i) r = fmaxf(r, sh[i].r);
+        a = Sum{r, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const Sum b = move_sum(sh[i], r);
+            a.s += b.s;
+            a.w += b.w;
+        }
+    }
+    return a;
+}
+
+// (m, s, w): max, sum 2^u and sum u 2^u with u = (x - m) c, for the rows that Sum does not hold.  An empty set is
+// (LOWEST, 0, 0): a finite start, so that a -inf logit (u = -inf) and a row of the type's lowest value (u = 0)
+// both come out as they should.
+struct Soft {
+    float m, s, w;
+};
+__device__ __forceinline__ void soft_add(Soft& a, float x, float c) {
+    const float m = nmax(a.m, x);
+    const float d = nmax((a.m - m) * c, -1e30f), k = ex2(d);
+    const float u = (x - m) * c, e = ex2(u);
+    a.w = (k == 0.f ? 0.f : (a.w + d * a.s) * k) + e * nmax(u, -1000.f);
+    a.s = a.s * k + e;
+    a.m = m;
+}
+__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {
+    const float m = nmax(a.m, b.m);
+    const float da = nmax((a.m - m) * c, -1e30f), db = nmax((b.m - m) * c, -1e30f);
+    const float ka = ex2(da), kb = ex2(db);
+    Soft r;
+    r.m = m;
+    r.s = a.s * ka + b.s * kb;
+    r.w = (ka == 0.f ? 0.f : (a.w + da * a.s) * ka) + (kb == 0.f ? 0.f : (b.w + db * b.s) * kb);
+    return r;
+}
+__device__ __forceinline__ Soft wave_soft(Soft v, float c) {
+    for (int o = 32; o > 0; o >>= 1)
+        v = soft_join(v, Soft{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.w, o)}, c);
+    return v;
+}
+template <int TEAM>
+__device__ Soft team_soft(Soft v, float c, Soft* sh) {
+    v = wave_soft(v, c);
+    if constexpr (TEAM > 64) {
+        __syncthreads();  // sh may still be read as Sum
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = sh[0];
+        for (int i = 1; i < TEAM / 64; ++i) v = soft_join(v, sh[i], c);
+    }
+    return v;
+}
+
+// A row's statistics as the gradients use them: u = x c - ref, or (x - ref) c on a wide row; p = 2^(u - l2)
+struct Stat {
+    float ref, s, w;
+    bool wide;
+};
+__device__ __forceinline__ float u_of(float x, float ref, bool wide, float c) {
+    return wide ? (x - ref) * c : __builtin_fmaf(x, c, -ref);
+}
+// the log-probability of a logit, l2 = log2 of the row's sum
+__device__ __forceinline__ float logp_of(float x, const Stat& st, float l2, float c, float invT) {
+    if (st.wide) return (x - st.ref) * invT - LN2 * l2;
+    if (fabsf(x) > 1e30f) return x * invT - LN2 * (st.ref + l2);  // x c may pass f32 where x / T does not
+    return LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
+}
+// is this sum a row's (some probability, all numbers)?  An empty one is a row without a legal action, or a wide one.
+__device__ __forceinline__ bool plain_sum(const Sum& a) { return a.s > 0.f && a.s < INFINITY; }
+
+// order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
+__device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {
+    const unsigned b = __float_as_uint(x + 0.f);  // -0 -> +0
+    const unsigned k = x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return ((unsigned long long)k << 32) | (0xFFFFFFFFu - idx);
+}
+__device__ __forceinline__ float key_value(unsigned long long key) {
+    const unsigned k = (unsigned)(key >> 32);
+    return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+}
+__device__ __forceinline__ unsigned key_index(unsigned long long key) { return 0xFFFFFFFFu - (unsigned)key; }
 
 // ln s in f64 for f32 s > 0: s = 2^e f, f in [0.75, 1.5), ln f = 2 atanh(u), u = (f - 1) / (f + 1), |u| <= 0.2,
 // by its power series to u^15 (what is left is under 2e-13)
@@ -97,199 +321,546 @@ __device__ __forceinline__ double ln_f64(float s) {
     return 0.69314718055994530942 * e + 2.0 * u * t;
 }
 
-// (m, s, w): max, sum 2^u and sum u 2^u with u = (x - m) c.  An empty set is (LOWEST, 0, 0): a finite start,
-// so that a -inf logit (u = -inf) and a row of the type's lowest value (u = 0) both come out as they should.
-struct Soft {
-    float m, s, w;
+
+// ---- one pass over a row --------------------------------------------------------------------------
+// GROUP vectors of a thread at once: loads first, then the group's maximum, then its exponentials.
+// bound by HBM: 8 operations and one exponential for a 2-byte logit are half of what the chip can do while it
+// loads it.
+template <class T, int U>
+struct Loaded {
+    uint4 v[U];
 };
-__device__ __forceinline__ void soft_add(Soft& a, float x, float c) {
-    const float m = nmax(a.m, x);
-    const float d = nmax((a.m - m) * c, -1e30f), k = ex2(d);  // an earlier sum moved to the new maximum: u' = u + d
-    const float u = (x - m) * c, uc = nmax(u, -1000.f);
-    const float e = ex2(u);
-    a.w = (k == 0.f ? 0.f : (a.w + d * a.s) * k) + e * uc;
-    a.s = a.s * k + e;
-    a.m = m;
-}
-__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {
-    const float m = nmax(a.m, b.m);
-    const float da = nmax((a.m - m) * c, -1e30f), db = nmax((b.m - m) * c, -1e30f);
-    const float ka = ex2(da), kb = ex2(db);
-    Soft r;
-    r.m = m;
-    r.s = a.s * ka + b.s * kb;
-    r.w = (ka == 0.f ? 0.f : (a.w + da * a.s) * ka) + (kb == 0.f ? 0.f : (b.w + db * b.s) * kb);
-    return r;
+template <class T, int TEAM, int U>
+__device__ __forceinline__ void load_group(Loaded<T, U>& L, const T* x, int vi, int nvec) {
+    if (vi - team_tid<TEAM>() + TEAM * U <= nvec) {  // the whole team's
+#pragma unroll
+        for (int u = 0; u < U; ++u) L.v[u] = load16(x + (long long)(vi + u * TEAM) * VN<T>);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            L.v[u] = make_uint4(MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>);
+            if (vi + u * TEAM < nvec) L.v[u] = load16(x + (long long)(vi + u * TEAM) * VN<T>);
+        }
+    }
 }
 
-// order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
-__device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {
-    unsigned b = __float_as_uint(x + 0.f);  // -0 -> +0
-    unsigned k = x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return ((unsigned long long)k << 32) | (0xFFFFFFFFu - idx);
+// what the top alternatives need of a pass: each thread's best vector and the maximum of each of its groups (LDS)
+struct Best {
+    float v;
+    int last;  // the last index of the first vector that holds v
+};
+
+// `edit` may take elements out of a vector (set them to -inf): edit(vector, its elements), edit.one(index).
+struct NoEdit {
+    template <class F>
+    __device__ __forceinline__ void operator()(int, F*) const {}
+    __device__ __forceinline__ bool one(int) const { return false; }
+};
+
+template <class T, int TEAM, bool MASK, bool ENT, bool TOP, class Edit>
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx, Best& best,
+                                         float* gmax, const Edit& edit) {
+    constexpr int N = VN<T>;
+    const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
+    int g = 0;
+    for (int vi = tid; vi - tid < nvec; vi += step, ++g) {
+        Loaded<T, GROUP> L;
+        load_group<T, TEAM, GROUP>(L, x, vi, nvec);
+        float f[GROUP * N], vm[GROUP];
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) {
+            unpack<T>(L.v[u], f + u * N);
+            if constexpr (MASK)
+                if (vi + u * TEAM < nvec) apply_mask<T>(mk + (long long)(vi + u * TEAM) * N, f + u * N);
+            edit(vi + u * TEAM, f + u * N);
+            float m = f[u * N];
+#pragma unroll
+            for (int i = 1; i < N; ++i) m = nmax(m, f[u * N + i]);
+            vm[u] = m;
+            if constexpr (TOP) {
+                const bool up = m > best.v;
+                best.v = up ? m : best.v;
+                best.last = up ? (vi + u * TEAM) * N + N - 1 : best.last;
+            }
+        }
+        float gm = vm[0];
+#pragma unroll
+        for (int u = 1; u < GROUP; ++u) gm = nmax(gm, vm[u]);
+        mx = nmax(mx, gm);
+        if constexpr (TOP) gmax[g * TEAM + tid] = gm;
+        sum_group<ENT, GROUP * N>(a, f, gm, c);
+    }
+    const int rest = V - nvec * N, i = nvec * N + tid;  // the last, incomplete vector, an element a thread
+    float f[2] = {-INFINITY, -INFINITY};
+    if (tid < rest && (!MASK || mk[i]) && !edit.one(i)) f[0] = (float)x[i];
+    if constexpr (TOP) {
+        gmax[g * TEAM + tid] = f[0];
+        if (f[0] > best.v) best = Best{f[0], i};
+    }
+    mx = nmax(mx, f[0]);
+    if (rest) sum_group<ENT, 2>(a, f, f[0], c);
+}
+
+// the row again, an element at a time, for what Sum does not hold
+template <class T, int TEAM, class Skip>
+__device__ Soft soft_pass(const T* x, const uint8_t* mk, int V, float c, Soft* sh, Skip skip) {
+    Soft v{LOWEST, 0.f, 0.f};
+    for (int i = team_tid<TEAM>(); i < V; i += TEAM)
+        if ((!mk || mk[i]) && !skip(i)) soft_add(v, (float)x[i], c);
+    return team_soft<TEAM>(v, c, sh);
 }
 
 template <int TEAM>
-__device__ Soft block_soft(Soft v, float c, Soft* sh) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = soft_join(v, Soft{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.w, o)}, c);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int i = 1; i < TEAM / 64; ++i) v = soft_join(v, sh[i], c);
-    __syncthreads();
-    return v;
+__device__ __forceinline__ float team_max(float x, float* sh) {
+    x = wave_max(x);
+    if constexpr (TEAM > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = sh[0];
+        for (int i = 1; i < TEAM / 64; ++i) x = nmax(x, sh[i]);
+        __syncthreads();
+    }
+    return x;
 }
 
-// the k-th key of a row by radix selection over the 64-bit order (value, then index: no two are equal), a
-// histogram of 256 digits at a time; returns the smallest key among the top k (0 if fewer are alternatives)
+union Shared {  // one reduction at a time
+    Sum sum[16];
+    Soft soft[16];
+    float f[16];
+};
+
+// a row's statistics from its pass: as they are, or by the element-wise pass; an empty row has s = 0
+template <class T, int TEAM, class Skip>
+__device__ __forceinline__ Stat row_stat(Sum a, float mx, const T* x, const uint8_t* mk, int V, float c, Shared& sh,
+                                         bool again, Skip skip) {
+    a = team_sum<TEAM>(a, sh.sum);
+    if (!again) {
+        if (plain_sum(a)) return Stat{a.r, a.s, a.w, false};
+        if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat{0.f, 0.f, 0.f, false};
+    }
+    const Soft v = soft_pass<T, TEAM>(x, mk, V, c, sh.soft, skip);
+    return Stat{v.m, v.s, v.w, true};
+}
+
+// ---- the k largest of a row -----------------------------------------------------------------------
+// A lower bound of the k-th largest: the k-th largest of the threads' (or of 64 groups of threads') own best is one,
+// for each of those k has an element at least as large.  In the order (value, index) it stays sharp where values
+// are equal: k threads of a constant row bound it by the index.  Only the groups whose maximum reaches the bound are
+// read again (cached, some k of them), what of them reaches it are the candidates, and a candidate's rank is the
+// number of those before it.  Where the list overflows (the largest crowd into few threads) or a logit is no
+// number, the bound is found by radix selection over the whole order, eight digits of 256.
+template <int TEAM>
+struct TopShare {
+    static constexpr int CANDS = TEAM == 64 ? 512 : 1024, HITS = TEAM == 64 ? 256 : 512;
+    unsigned long long cand[CANDS];  // before: the threads' best; in the radix selection: the histogram
+    int hits[HITS];
+    int nh, nc;
+    unsigned long long bound;
+};
+
+template <int G>
+__device__ __forceinline__ int rank_in(const unsigned long long* arr, unsigned long long me) {
+    int rank = 0;
+#pragma unroll 16
+    for (int i = 0; i < G; ++i) rank += arr[i] > me;
+    return rank;
+}
+
+template <int TEAM>
+__device__ __forceinline__ unsigned long long kth_best(unsigned long long best, int k, TopShare<TEAM>& S) {
+    const int tid = team_tid<TEAM>(), lane = threadIdx.x & 63;
+    unsigned long long* arr = S.cand;
+    if (tid == 0) S.nh = 0, S.nc = 0, S.bound = 0;
+    if (TEAM == 64 || k <= 32) {  // 64 groups of TEAM / 64 threads, every wave for itself
+        if (k > 64) {
+            team_sync<TEAM>();
+            return 0;
+        }
+        auto mx = [](unsigned long long a, unsigned long long b) { return a > b ? a : b; };
+        constexpr int P = TEAM / 64;
+        if constexpr (P >= 2) best = mx(best, dpp<QUAD_XOR1>(best));
+        if constexpr (P >= 4) best = mx(best, dpp<QUAD_XOR2>(best));
+        static_assert(P <= 4, "groups of at most a quad");
+        if (P == 1 || (tid & (P - 1)) == 0) arr[tid / P] = best;
+        team_sync<TEAM>();
+        const unsigned long long me = arr[lane];
+        const int rank = rank_in<64>(arr, me);
+        const unsigned long long at = __ballot(me != 0 && rank == k - 1);
+        if (TEAM > 64) __syncthreads();  // arr becomes the candidates
+        return at ? lane_of(me, __builtin_ctzll(at)) : 0;
+    }
+    arr[tid] = best;
+    team_sync<TEAM>();
+    if (best != 0 && rank_in<TEAM>(arr, best) == k - 1) S.bound = best;
+    team_sync<TEAM>();
+    return S.bound;
+}
+
 template <class T, int TEAM>
 __device__ unsigned long long radix_kth(const T* x, const uint8_t* mk, int V, int k, unsigned* hist) {
     unsigned long long prefix = 0;
     int need = k;
     for (int d = 7; d >= 0; --d) {
-        for (int i = threadIdx.x; i < 256; i += TEAM) hist[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < V; i += TEAM) {
+        for (int i = team_tid<TEAM>(); i < 256; i += TEAM) hist[i] = 0;
+        team_sync<TEAM>();
+        for (int i = team_tid<TEAM>(); i < V; i += TEAM) {
             const float v = (float)x[i];
             if ((mk && !mk[i]) || v == -INFINITY) continue;
             const unsigned long long key = order_key(v, i);
             if (d < 7 && (key >> (8 * d + 8)) != (prefix >> (8 * d + 8))) continue;
             atomicAdd(&hist[(key >> (8 * d)) & 255], 1u);
         }
-        __syncthreads();
+        team_sync<TEAM>();
         int bin = 255, above = 0;
         for (; bin >= 0; --bin) {  // every thread walks the same counts
             const int n = hist[bin];
             if (above + n >= need) break;
             above += n;
         }
-        __syncthreads();
-        if (bin < 0) return prefix;  // fewer than k: all of them (only possible at the first digit)
+        team_sync<TEAM>();
+        if (bin < 0) return 0;  // fewer than k: all of them (only possible at the first digit)
         prefix |= (unsigned long long)bin << (8 * d);
         need -= above;
     }
     return prefix;
 }
 
+// the candidates by radix selection: exactly min(k, alternatives) of them
+template <class T, int TEAM>
+__device__ int radix_select(const T* x, const uint8_t* mk, int V, int k, TopShare<TEAM>& S) {
+    const int tid = team_tid<TEAM>();
+    team_sync<TEAM>();
+    const unsigned long long lo = radix_kth<T, TEAM>(x, mk, V, k, (unsigned*)S.cand);
+    if (tid == 0) S.nc = 0;
+    team_sync<TEAM>();
+    for (int i = tid; i < V; i += TEAM) {
+        const float f = (float)x[i];
+        if ((mk && !mk[i]) || f == -INFINITY) continue;
+        const unsigned long long key = order_key(f, i);
+        if (key >= lo) S.cand[atomicAdd(&S.nc, 1)] = key;
+    }
+    team_sync<TEAM>();
+    return S.nc;
+}
+
+template <class T, int TEAM, bool MASK>
+__device__ int top_select(const T* x, const uint8_t* mk, int V, int k, bool plain, Best b, const float* gmax,
+                          TopShare<TEAM>& S) {
+    constexpr int N = VN<T>;
+    const int tid = team_tid<TEAM>(), nvec = V / N, ng = (nvec + TEAM * GROUP - 1) / (TEAM * GROUP);
+    if (plain) {  // uniform over the team
+        const unsigned long long bound = kth_best<TEAM>(b.v > -INFINITY ? order_key(b.v, b.last) : 0, k, S);
+        const float bv = bound ? key_value(bound) : LOWEST;
+        for (int g = 0; g <= ng; ++g) {
+            const float gm = gmax[g * TEAM + tid];
+            if (gm >= bv) {
+                const int h = atomicAdd(&S.nh, 1);
+                if (h < S.HITS) S.hits[h] = g * TEAM + tid;
+            }
+        }
+        team_sync<TEAM>();
+        const int nh = S.nh;
+        if (nh <= S.HITS) {
+            for (int i = tid; i < nh * GROUP; i += TEAM) {
+                const int h = S.hits[i / GROUP], u = i % GROUP, g = h / TEAM, t = h % TEAM;
+                float f[N];
+                int i0, n = 0;
+                if (g == ng) {
+                    i0 = nvec * N + t;
+                    if (u == 0) {
+                        f[0] = (float)x[i0];
+                        n = 1;
+                    }
+                } else {
+                    const int vi = (g * GROUP + u) * TEAM + t;
+                    i0 = vi * N;
+                    if (vi < nvec) {
+                        unpack<T>(load16(x + i0), f);
+                        if constexpr (MASK) apply_mask<T>(mk + i0, f);
+                        n = N;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (j >= n || !(f[j] >= bv)) continue;
+                    const unsigned long long key = order_key(f[j], i0 + j);
+                    if (key < bound) continue;
+                    const int at = atomicAdd(&S.nc, 1);
+                    if (at < S.CANDS) S.cand[at] = key;
+                }
+            }
+            team_sync<TEAM>();
+            const int n = S.nc;
+            if (n <= S.CANDS) return n;
+        }
+    }
+    return radix_select<T, TEAM>(x, mk, V, k, S);
+}
+
+// out(rank, key) of the first k candidates, out(rank, 0) where there are fewer
+template <int TEAM, class Out>
+__device__ __forceinline__ void top_out(const TopShare<TEAM>& S, int n, int k, Out out) {
+    const int tid = team_tid<TEAM>();
+    for (int i = tid; i < n; i += TEAM) {
+        const unsigned long long me = S.cand[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += S.cand[j] > me;
+        if (rank < k) out(rank, me);
+    }
+    for (int j = n + tid; j < k; j += TEAM) out(j, 0ull);
+}
+
+// ---- log-probabilities ------------------------------------------------------------------------------
+struct LogprobsOut {
+    const void* actions;
+    int act64, k;
+    float *stats, *logp, *entropy, *lse, *top_logp;
+    long long* top_ids;
+};
+
+// a row's given action: its index is read ahead of the pass, its logit (by then cached) after it
+__device__ __forceinline__ long long action_of(const LogprobsOut& O, long long r) {
+    if (!O.logp) return -1;
+    return O.act64 ? ((const long long*)O.actions)[r] : ((const int*)O.actions)[r];
+}
+
+template <class T>
+__device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat& st, float l2,
+                                          long long act, const T* x, const uint8_t* mk) {
+    const bool empty = st.s == 0.f;
+    const float H = empty ? 0.f : LN2 * (l2 - st.w / st.s);
+    if (O.stats) ((float4*)O.stats)[r] = make_float4(st.ref, st.s, H, st.wide ? 1.f : 0.f);
+    O.entropy[r] = H;
+    O.lse[r] = empty ? -INFINITY : st.wide ? st.ref * R.invT + LN2 * l2 : LN2 * (st.ref + l2);
+    if (O.logp) {
+        float p = 0.f;
+        if (act >= 0 && act < R.V) {
+            p = empty || (mk && !mk[act]) ? -INFINITY : logp_of((float)x[act], st, l2, R.c, R.invT);
+            if (st.s != st.s) p = st.s;
+        }
+        O.logp[r] = p;
+    }
+}
+
+// a part of a row for rows split over blocks: (r, s, w, 1 if it has to be done again as a wide row)
+struct Split {
+    float4* part;               // [rows][n]
+    unsigned long long* keys;   // [rows][n][k], by rank, 0: none
+    int n, len;                 // parts, elements in each but the last
+};
+
+template <class T, int TEAM, bool MASK, bool TOP, bool PART>
+__global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, LogprobsOut O, Split P) {
+    extern __shared__ float gmax_all[];
+    constexpr int TEAMS = block_of<TEAM> / TEAM;
+    __shared__ Shared sh;
+    __shared__ TopShare<TEAM> tops[TOP ? TEAMS : 1];
+    const long long r = team_row<TEAM>();
+    if (r >= R.rows) return;
+    const T* x = row_ptr<T>(R, r);
+    const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
+    const int tid = team_tid<TEAM>();
+    int V = R.V, from = 0;
+    if constexpr (PART) {
+        from = blockIdx.z * P.len;
+        V = V - from < P.len ? V - from : P.len;
+        x += from;
+        if constexpr (MASK) mk += from;
+    }
+    const int ng = (V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP);
+    float* gmax = gmax_all + team_in_block<TEAM>() * (ng + 1) * TEAM;
+    long long act = -1;
+    if constexpr (!PART) act = action_of(O, r);
+    Sum a{-FAR, 0.f, 0.f};
+    float mx = -INFINITY;
+    Best best{-INFINITY, 0};
+    row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{});
+    Stat st;
+    float l2 = 0.f;
+    if constexpr (PART) {
+        a = team_sum<TEAM>(a, sh.sum);
+        const bool plain = plain_sum(a);
+        const float all = plain ? 0.f : team_max<TEAM>(mx, sh.f);
+        st.wide = !plain && all != -INFINITY;
+        if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, plain ? a.w : 0.f, st.wide);
+    } else {
+        st = row_stat<T, TEAM>(a, mx, x, mk, V, R.c, sh, false, [](int) { return false; });
+        l2 = lg2(st.s);
+        if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
+    }
+    if constexpr (TOP) {
+        TopShare<TEAM>& S = tops[team_in_block<TEAM>()];
+        const int n = top_select<T, TEAM, MASK>(x, mk, V, O.k, !st.wide, best, gmax, S);
+        top_out<TEAM>(S, n, O.k, [&](int rank, unsigned long long key) {
+            if constexpr (PART) {
+                // the index within the row: the key holds its complement
+                P.keys[((long long)r * P.n + blockIdx.z) * O.k + rank] = key ? key - from : 0;
+            } else {
+                O.top_ids[r * O.k + rank] = key ? (long long)key_index(key) : -1;
+                O.top_logp[r * O.k + rank] =
+                    key ? logp_of(key_value(key), st, l2, R.c, R.invT) : -INFINITY;
+            }
+        });
+    }
+}
+
+// the parts of a row joined
 template <class T, bool TOP>
-__global__ __launch_bounds__(256) void logprobs_rows_kernel(Rows R, const void* actions, int act64, int k,
-                                                            float* __restrict__ stats, float* __restrict__ logp,
-                                                            float* __restrict__ entropy, float* __restrict__ lse,
-                                                            float* __restrict__ top_logp,
-                                                            long long* __restrict__ top_ids) {
-    __shared__ Soft sh[4];
-    __shared__ unsigned hist[256];
-    __shared__ unsigned long long cand[TOP_MAX];
-    __shared__ unsigned ncand;
+__global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut O, Split P) {
+    __shared__ Shared sh;
+    __shared__ TopShare<256> S;
     const long long r = block_row();
     if (r >= R.rows) return;
     const T* x = row_ptr<T>(R, r);
     const uint8_t* mk = mask_ptr(R, r);
     const int tid = threadIdx.x;
-    Soft v{LOWEST, 0.f, 0.f};
-    for (int i = tid; i < R.V; i += 256)
-        if (!mk || mk[i]) soft_add(v, (float)x[i], R.c);
-    v = block_soft<256>(v, R.c, sh);
-    const float l2 = __builtin_amdgcn_logf(v.s);
-    if (tid == 0) {
-        const bool empty = v.s == 0.f;
-        const float H = empty ? 0.f : LN2 * (l2 - v.w / v.s);
-        if (stats) {
-            stats[4 * r] = v.m;
-            stats[4 * r + 1] = l2;
-            stats[4 * r + 2] = H;
-        }
-        entropy[r] = H;
-        lse[r] = empty ? -INFINITY : v.m * R.invT + LN2 * l2;
-        if (logp) {
-            const long long a = act64 ? ((const long long*)actions)[r] : ((const int*)actions)[r];
-            float p = 0.f;
-            if (a >= 0 && a < R.V) {
-                p = empty || (mk && !mk[a]) ? -INFINITY : ((float)x[a] - v.m) * R.invT - LN2 * l2;
-                if (v.s != v.s) p = v.s;
-            }
-            logp[r] = p;
-        }
+    const long long act = action_of(O, r);
+    Sum a{-FAR, 0.f, 0.f};
+    bool again = false;
+    for (int i = tid; i < P.n; i += 256) {
+        const float4 p = P.part[r * P.n + i];
+        const float m = fmaxf(a.r, p.x);
+        const Sum b = move_sum(Sum{p.x, p.y, p.z}, m);
+        a = move_sum(a, m);
+        a.s += b.s;
+        a.w += b.w;
+        again |= p.w != 0.f;
     }
+    unsigned long long best = 0;
+    const unsigned long long* keys = nullptr;
+    const int nk = P.n * O.k;
     if constexpr (TOP) {
-        const unsigned long long lo = radix_kth<T, 256>(x, mk, R.V, k, hist);
-        if (tid == 0) ncand = 0;
-        __syncthreads();
-        for (int i = tid; i < R.V; i += 256) {
-            const float f = (float)x[i];
-            if ((mk && !mk[i]) || f == -INFINITY) continue;
-            const unsigned long long key = order_key(f, i);
-            if (key >= lo) cand[atomicAdd(&ncand, 1u)] = key;
+        keys = P.keys + r * nk;
+        for (int i = tid; i < nk; i += 256) best = best > keys[i] ? best : keys[i];
+    }
+    again = __syncthreads_or(again);
+    Stat st;
+    if (again) {
+        const Soft v = soft_pass<T, 256>(x, mk, R.V, R.c, sh.soft, [](int) { return false; });
+        st = Stat{v.m, v.s, v.w, true};
+    } else {
+        a = team_sum<256>(a, sh.sum);
+        st = Stat{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
+    }
+    const float l2 = lg2(st.s);
+    if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
+    if constexpr (TOP) {
+        const unsigned long long bound = kth_best<256>(best, O.k, S);
+        for (int i = tid; i < nk; i += 256) {
+            const unsigned long long key = keys[i];
+            if (key == 0 || key < bound) continue;
+            const int at = atomicAdd(&S.nc, 1);
+            if (at < S.CANDS) S.cand[at] = key;
         }
         __syncthreads();
-        const int n = ncand;
-        for (int j = tid; j < k; j += 256) {
-            if (j < n) {
-                const unsigned long long me = cand[j];
-                int rank = 0;
-                for (int i = 0; i < n; ++i) rank += cand[i] > me;
-                const unsigned id = 0xFFFFFFFFu - (unsigned)me;
-                top_ids[r * k + rank] = id;
-                top_logp[r * k + rank] = ((float)x[id] - v.m) * R.invT - LN2 * l2;
-            } else {
-                top_ids[r * k + j] = -1;
-                top_logp[r * k + j] = -INFINITY;
-            }
-        }
+        int n = S.nc;
+        if (n > S.CANDS) n = radix_select<T, 256>(x, mk, R.V, O.k, S);
+        top_out<256>(S, n, O.k, [&](int rank, unsigned long long key) {
+            O.top_ids[r * O.k + rank] = key ? (long long)key_index(key) : -1;
+            O.top_logp[r * O.k + rank] = key ? logp_of(key_value(key), st, l2, R.c, R.invT) : -INFINITY;
+        });
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void logprobs_bwd_kernel(Rows R, const void* actions, int act64,
+// Elementwise over a row or a part of it: f(x, legal) for each element, vectors of 16 bytes.  Rows are taken from
+// the last to the first: what a forward pass read last may still be in the Infinity Cache.
+template <class T, int TEAM, bool MASK, class F>
+__device__ __forceinline__ void map_row(const T* x, const uint8_t* mk, T* d, int V, F f) {
+    constexpr int N = VN<T>;
+    const int tid = team_tid<TEAM>(), nvec = V / N;
+    for (int vi = tid; vi - tid < nvec; vi += TEAM * GROUP) {
+        Loaded<T, GROUP> L;
+        load_group<T, TEAM, GROUP>(L, x, vi, nvec);
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) {
+            const int i0 = (vi + u * TEAM) * N;
+            if (vi + u * TEAM >= nvec) continue;
+            float y[N];
+            unpack<T>(L.v[u], y);
+            if constexpr (MASK) {
+                uint8_t b[N];
+                __builtin_memcpy(b, mk + i0, N);
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = b[i] ? f(y[i], i0 + i) : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = f(y[i], i0 + i);
+            }
+            store16(d + i0, y);
+        }
+    }
+    const int i = nvec * N + tid;
+    if (i < V) d[i] = (T)(!MASK || mk[i] ? f((float)x[i], i) : 0.f);
+}
+
+template <class T, int TEAM, bool MASK>
+__global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, const void* actions, int act64,
                                                            const float* __restrict__ stats, const float* gl,
                                                            long long gl_s, const float* ge, long long ge_s,
-                                                           const float* gz, long long gz_s, T* __restrict__ dx) {
-    const long long r = block_row();
-    if (r >= R.rows) return;
-    const T* x = row_ptr<T>(R, r);
-    const uint8_t* mk = mask_ptr(R, r);
-    const float m = stats[4 * r], l2 = stats[4 * r + 1], H = stats[4 * r + 2];
+                                                           const float* gz, long long gz_s, T* __restrict__ dx,
+                                                           int len) {
+    const long long r = R.rows - 1 - team_row<TEAM>();
+    if (r < 0) return;
+    const int from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
+    const T* x = row_ptr<T>(R, r) + from;
+    const uint8_t* mk = MASK ? mask_ptr(R, r) + from : nullptr;
+    const float4 st = ((const float4*)stats)[r];
+    const float ref = st.x, s = st.y, H = st.z;
     long long a = -1;
     if (actions) a = act64 ? ((const long long*)actions)[r] : ((const int*)actions)[r];
     const bool given = a >= 0 && a < R.V;
     const float g1 = gl && given ? gl[r * gl_s] : 0.f, g2 = ge ? ge[r * ge_s] : 0.f, g3 = gz ? gz[r * gz_s] : 0.f;
-    const float c0 = (g3 - g1 - g2 * H) * R.invT, c1 = g2 * R.invT * LN2, ga = g1 * R.invT;
-    T* d = dx + r * (long long)R.V;
-    const bool empty = l2 == -INFINITY;
-    for (int i = threadIdx.x; i < R.V; i += 256) {
-        float g = 0.f;
-        if (!empty && (!mk || mk[i])) {
-            const float z = nmax(((float)x[i] - m) * R.c - l2, -1000.f);
-            g = ex2(z) * (c0 - c1 * z);
-            if (i == a) g += ga;
-        }
-        d[i] = (T)g;
+    // p = 2^u / s and ln p = ln2 (u - log2 s): dx = 2^u (c0 - c1 u)
+    const float c1 = g2 * R.invT * LN2 / s, ga = g1 * R.invT;
+    const float c0 = (g3 - g1 - g2 * H) * R.invT / s + c1 * lg2(s);
+    T* d = dx + r * (long long)R.V + from;
+    const int at = given ? (int)(a - from) : -1;  // outside this part: no element's index
+    if (s == 0.f) {  // no legal action
+        map_row<T, TEAM, false>(x, mk, d, V, [](float, int) { return 0.f; });
+    } else if (st.w != 0.f) {
+        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int i) {
+            const float u = nmax((y - ref) * R.c, -1000.f);
+            return ex2(u) * (c0 - c1 * u) + (i == at ? ga : 0.f);
+        });
+    } else {
+        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int i) {
+            const float u = nmax(__builtin_fmaf(y, R.c, -ref), -1000.f);
+            const float g = ex2(u) * __builtin_fmaf(-c1, u, c0);
+            return i == at ? g + ga : g;
+        });
     }
 }
 
-// ---- distillation ---------------------------------------------------------------------------
-
+// ---- distillation ---------------------------------------------------------------------------------------
 struct Teacher {
     const void* logp;
     const void* ids;
     int dtype, ids64, k, rest;
 };
 
-// a row's teacher entries, by its first wave: ids (-1: none), t, q, and tm, qs with q = exp(t - tm) / qs (rest: exp t)
+// a row's teacher entries: ids (-1: none), the student's logits there (illegal: -inf), t, q = exp(t - tm) / qs (rest:
+// exp t); first: no earlier entry has the same id
 struct Entries {
     int id[TOP_MAX];
-    float t[TOP_MAX], q[TOP_MAX];
+    float x[TOP_MAX], t[TOP_MAX], q[TOP_MAX];
+    bool first[TOP_MAX];
+};
+struct EntryHead {
     float tm, qs;
-    int any;
+    bool any, far;  // far: a student's logit that Sum does not hold
 };
 
-__device__ void load_entries(Entries& E, const Teacher& Te, long long r, int V) {
+// by one wave, an entry or two a lane
+template <class T>
+__device__ __forceinline__ EntryHead load_entries(Entries& E, const Teacher& Te, long long r, int V, const T* x,
+                                                  const uint8_t* mk, float c) {
     const int lane = threadIdx.x & 63;
     float tm = -INFINITY;
     float t[2];
     int id[2];
+    bool far = false;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
@@ -305,6 +876,12 @@ __device__ void load_entries(Entries& E, const Teacher& Te, long long r, int V) 
                 id[u] = (int)i;
                 t[u] = f;
             }
+            float xj = -INFINITY;
+            if (id[u] >= 0 && (!mk || mk[id[u]])) xj = (float)x[id[u]];
+            E.id[j] = id[u];
+            E.t[j] = t[u];
+            E.x[j] = xj;
+            far |= xj != -INFINITY && !(fabsf(xj * c) < FAR);
         }
         tm = nmax(tm, t[u]);
     }
@@ -319,60 +896,69 @@ __device__ void load_entries(Entries& E, const Teacher& Te, long long r, int V) 
     }
     qs = wave_sum(qs);
     const float iq = Te.rest || !any ? 1.f : 1.f / qs;
+    team_sync<64>();
+    bool dup[2] = {false, false};
+    if (Te.rest)
+        for (int i = 0; i + 1 < Te.k; ++i) {
+            const int e = E.id[i];
+            dup[0] |= i < lane && e == id[0];
+            dup[1] |= i < lane + 64 && e == id[1];
+        }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
         if (j < Te.k) {
-            E.id[j] = id[u];
-            E.t[j] = t[u];
             E.q[j] = q[u] * iq;
+            E.first[j] = !dup[u];
         }
     }
-    if (lane == 0) {
-        E.tm = tm;
-        E.qs = qs;
-        E.any = any;
-    }
+    team_sync<64>();
+    return EntryHead{tm, qs, any, __ballot(far) != 0};
 }
 
-// is an earlier entry of the row this one's id as well
-__device__ __forceinline__ bool earlier(const Entries& E, int j) {
-    for (int i = 0; i < j; ++i)
-        if (E.id[i] == E.id[j]) return true;
-    return false;
-}
-
-struct Row {  // what the gradient needs of a row: with e(x, m, l) = 2^((x - m) c - l)
-    float mo, lo, b;  // dx = b e(x, mo, lo) w / T, but
-    float m, l, a;    // dx = (a e(x, m, l) - q) w / T at the entries
-    float pad[2];
+struct Row {  // what the gradient needs of a row: p(x, ref, s) = 2^u(x, ref) / s
+    float ro, so, b;  // dx = b p(x, ro, so) w / T, but
+    float ra, sa, a;  // dx = (a p(x, ra, sa) - q) w / T at the entries
+    float wide, pad;
 };
 
-// one row's loss and coefficients by the first wave, from the student's statistics over all legal actions outside
-// the entries (rest) or over all (else)
-template <class T>
-__device__ float finish_row(const Rows& R, const Teacher& Te, const Entries& E, Soft v, const T* x,
-                            const uint8_t* mk, Row* out) {
+// one row's loss and coefficients, by one wave, from the student's statistics over all legal actions outside the
+// entries (rest) or over all (else)
+__device__ __forceinline__ Row finish_row(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
+                                          const Stat& v, float* row_loss) {
     const int lane = threadIdx.x & 63;
     float xj[2];
     bool ok[2];
-    Soft e{LOWEST, 0.f, 0.f};
+    float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
         ok[u] = j < Te.k && E.id[j] >= 0;
-        xj[u] = ok[u] && (!mk || mk[E.id[j]]) ? (float)x[E.id[j]] : -INFINITY;
-        if (Te.rest && ok[u] && !earlier(E, j)) soft_add(e, xj[u], R.c);
+        xj[u] = ok[u] ? E.x[j] : -INFINITY;
+        mx = nmax(mx, xj[u]);
     }
-    Soft all = v;
+    Stat all = v;
     if (Te.rest) {
+        mx = wave_max(mx);
+        Stat e{0.f, 0.f, 0.f, v.wide};
+        if (mx != -INFINITY) {
+            e.ref = v.wide ? mx : rintf(mx * R.c);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            e = soft_join(e, Soft{__shfl_xor(e.m, o), __shfl_xor(e.s, o), __shfl_xor(e.w, o)}, R.c);
-        all = soft_join(v, e, R.c);
+            for (int u = 0; u < 2; ++u)
+                if (ok[u] && E.first[lane + 64 * u]) e.s += ex2(u_of(xj[u], e.ref, v.wide, R.c));
+            e.s = wave_sum(e.s);
+        }
+        if (e.s != 0.f && v.s != 0.f) {
+            all.ref = nmax(e.ref, v.ref);
+            const float de = v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref;
+            const float dv = v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref;
+            all.s = e.s * ex2(de) + v.s * ex2(dv);
+        } else if (e.s != 0.f) {
+            all = e;
+        }
     }
-    const double invT = (double)R.c * 0.69314718055994530942;
-    const double lns = ln_f64(all.s), lnq = Te.rest ? 0.0 : ln_f64(E.qs);
+    const double cd = R.c, ln2 = 0.69314718055994530942;
+    const double lns = ln_f64(all.s), lnq = Te.rest ? 0.0 : ln_f64(h.qs);
     double loss = 0.0, Q = 0.0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -380,8 +966,9 @@ __device__ float finish_row(const Rows& R, const Teacher& Te, const Entries& E, 
         const int j = lane + 64 * u;
         const double q = E.q[j];
         Q += q;
-        const double lq = ((double)E.t[j] - (double)E.tm) - lnq;
-        const double lp = ((double)xj[u] - (double)all.m) * invT - lns;
+        const double lq = ((double)E.t[j] - (double)h.tm) - lnq;
+        const double uj = v.wide ? ((double)xj[u] - (double)all.ref) * cd : (double)xj[u] * cd - (double)all.ref;
+        const double lp = uj * ln2 - lns;
         if (q > 0.0 || q != q) loss += q * (lq - lp);
     }
     loss = wave_sum(loss);
@@ -390,95 +977,303 @@ __device__ float finish_row(const Rows& R, const Teacher& Te, const Entries& E, 
     if (Te.rest) {
         pr = 0.0;
         if (v.s != 0.f) {
-            const double lpr = ((double)v.m - (double)all.m) * invT + ln_f64(v.s) - lns;
-            pr = exp(lpr);
+            const double d = v.wide ? ((double)v.ref - (double)all.ref) * cd : (double)v.ref - (double)all.ref;
+            const double lpr = d * ln2 + ln_f64(v.s) - lns;
+            const double y = lpr * 1.4426950408889634074, yi = rint(y);
+            pr = (double)__builtin_amdgcn_ldexpf(ex2((float)(y - yi)), (int)fmax(yi, -4096.0));
+            if (lpr != lpr) pr = lpr;
             qr = 1.0 - Q;
             if (qr < 0.0) qr = 0.0;
             if (qr != 0.0) loss += qr * (ln_f64((float)qr) - lpr);
             S += qr;
         }
     }
-    const bool none = !E.any || all.s == 0.f;
-    if (none) loss = 0.0, S = 0.0, qr = 0.0;
-    if (lane == 0) {
-        out->mo = v.m;
-        out->lo = v.s == 0.f ? 0.f : __builtin_amdgcn_logf(v.s);
-        out->b = (float)(S * pr - qr);
-        out->m = all.m;
-        out->l = all.s == 0.f ? 0.f : __builtin_amdgcn_logf(all.s);
-        out->a = (float)S;
-    }
-    return (float)loss;
+    if (!h.any || all.s == 0.f) loss = 0.0, S = 0.0, qr = 0.0;
+    if (lane == 0 && row_loss) *row_loss = (float)loss;
+    return Row{v.ref, v.s, (float)(S * pr - qr), all.ref, all.s, (float)S, v.wide ? 1.f : 0.f, 0.f};
 }
 
+// the entries of a row as bits, an element each: what a pass leaves out
 template <class T>
-__global__ __launch_bounds__(256) void distill_rows_kernel(Rows R, Teacher Te, float* __restrict__ stats,
-                                                           float* __restrict__ row_loss) {
-    constexpr int CH = 65536;  // elements between two settings of the bitmap of entries
-    __shared__ Soft sh[4];
-    __shared__ Entries E;
-    __shared__ unsigned bits[CH / 32];
-    const long long r = block_row();
-    if (r >= R.rows) return;
-    const T* x = row_ptr<T>(R, r);
-    const uint8_t* mk = mask_ptr(R, r);
-    const int tid = threadIdx.x;
-    if (tid < 64) load_entries(E, Te, r, R.V);
-    Soft v{LOWEST, 0.f, 0.f};
-    for (int c0 = 0; c0 < R.V; c0 += CH) {
-        const int n = R.V - c0 < CH ? R.V - c0 : CH;
-        if (Te.rest) {
-            __syncthreads();
-            for (int i = tid; i < (n + 31) / 32; i += 256) bits[i] = 0;
-            __syncthreads();
-            for (int j = tid; j < Te.k; j += 256) {
-                const int i = E.id[j] - c0;
-                if (E.id[j] >= 0 && i >= 0 && i < n) atomicOr(&bits[i >> 5], 1u << (i & 31));
-            }
-            __syncthreads();
-        }
-        for (int i = tid; i < n; i += 256)
-            if ((!mk || mk[c0 + i]) && !(Te.rest && (bits[i >> 5] >> (i & 31) & 1))) soft_add(v, (float)x[c0 + i], R.c);
-    }
-    v = block_soft<256>(v, R.c, sh);
-    if (tid < 64) {
-        Row o;
-        const float loss = finish_row<T>(R, Te, E, v, x, mk, &o);
-        if (tid == 0) {
-            row_loss[r] = loss;
-            if (stats) ((Row*)stats)[r] = o;
+struct SkipBits {
+    const unsigned* bits;
+    bool on;
+    __device__ __forceinline__ void operator()(int vi, float* f) const {
+        if (!on) return;
+        constexpr int N = VN<T>;
+        unsigned b = ((const uint8_t*)bits)[N == 8 ? vi : vi >> 1];
+        if (N == 4) b = (b >> (4 * (vi & 1))) & 15;
+        if (b) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = (b >> i) & 1 ? -INFINITY : f[i];
         }
     }
+    __device__ __forceinline__ bool one(int i) const { return on && (bits[i >> 5] >> (i & 31) & 1); }
+};
+// words of the bitmap: whole groups of vectors may be looked up past the row's end
+template <class T, int TEAM>
+__host__ __device__ constexpr int bit_words(int V) {
+    return (V / VN<T> / (TEAM * GROUP) + 1) * TEAM * GROUP * VN<T> / 32 + 1;
+}
+__device__ __forceinline__ void set_bit(unsigned* bits, int id, int from, int V) {
+    const int i = id - from;
+    if (id >= 0 && i >= 0 && i < V) atomicOr(&bits[i >> 5], 1u << (i & 31));
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void distill_bwd_kernel(Rows R, Teacher Te, const float* __restrict__ stats,
-                                                          const float* w, long long w_s, float w0,
-                                                          T* __restrict__ dx) {
-    __shared__ Entries E;
-    const long long r = block_row();
-    if (r >= R.rows) return;
-    const T* x = row_ptr<T>(R, r);
-    const uint8_t* mk = mask_ptr(R, r);
-    const int tid = threadIdx.x;
-    const Row st = ((const Row*)stats)[r];
-    const float g = (w ? w[r * w_s] : 1.f) * w0 * R.invT;
-    T* d = dx + r * (long long)R.V;
-    if (tid < 64) load_entries(E, Te, r, R.V);
-    for (int i = tid; i < R.V; i += 256) {
-        float f = 0.f;
-        if (!mk || mk[i]) f = ex2(((float)x[i] - st.mo) * R.c - st.lo) * st.b * g;
-        d[i] = (T)f;
-    }
-    __syncthreads();
-    for (int j = tid; j < Te.k; j += 256) {
-        const int id = E.id[j];
-        if (id < 0 || (mk && !mk[id])) continue;
+// the entries' elements of a row (or a part of it), after all its elements
+template <class T, int TEAM>
+__device__ __forceinline__ void write_entries(const Rows& R, const Teacher& Te, const Entries& E, const Row& o, float g,
+                                              const uint8_t* mk, T* d, int from, int V) {
+    for (int j = team_tid<TEAM>(); j < Te.k; j += TEAM) {
+        const int id = E.id[j], i = id - from;
+        if (id < 0 || i < 0 || i >= V || (mk && !mk[i])) continue;
         float q = 0.f;  // the same index twice: its entries' probabilities add
-        for (int i = 0; i < Te.k; ++i) q += E.id[i] == id ? E.q[i] : 0.f;
-        if (st.a == 0.f) q = 0.f;  // a row without a legal action
-        d[id] = (T)((ex2(((float)x[id] - st.m) * R.c - st.l) * st.a - q) * g);
+        for (int e = 0; e < Te.k; ++e) q += E.id[e] == id ? E.q[e] : 0.f;
+        const float p = ex2(u_of(E.x[j], o.ra, o.wide != 0.f, R.c)) * (o.a / o.sa);
+        d[i] = (T)(o.a == 0.f ? 0.f : (p - q) * g);  // a = 0: a row without a legal action
     }
+}
+
+template <class T, int TEAM, bool MASK>
+__device__ __forceinline__ void write_outside(const Rows& R, const Row& o, float g, const T* x, const uint8_t* mk, T* d,
+                                              int V) {
+    const float b = o.so == 0.f ? 0.f : o.b * g / o.so;
+    if (o.so == 0.f)
+        map_row<T, TEAM, false>(x, mk, d, V, [](float, int) { return 0.f; });
+    else if (o.wide != 0.f)
+        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int) { return ex2((y - o.ro) * R.c) * b; });
+    else
+        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int) { return ex2(__builtin_fmaf(y, R.c, -o.ro)) * b; });
+}
+
+struct DistillOut {
+    float *stats, *row_loss;
+    const float* w;
+    long long w_s;
+    float scale;
+    void* dx;
+};
+__device__ __forceinline__ float row_weight(const Rows& R, const DistillOut& O, long long r) {
+    return (O.w ? O.w[r * O.w_s] : 1.f) * O.scale * R.invT;
+}
+
+// A team a row: statistics, loss and (dx) the gradient.  NV > 0: the row stays in registers (NV vectors a thread)
+// between its two uses, and HBM sees it once; NV = 0: it is read again from the cache.
+template <class T, int TEAM, bool MASK, int NV>
+__global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
+    extern __shared__ unsigned bits_all[];
+    constexpr int TEAMS = block_of<TEAM> / TEAM, N = VN<T>;
+    __shared__ Shared sh;
+    __shared__ Entries Es[TEAMS];
+    __shared__ Row rows[TEAMS];
+    __shared__ bool fars[TEAMS];
+    const long long r = team_row<TEAM>();
+    if (r >= R.rows) return;
+    const T* x = row_ptr<T>(R, r);
+    const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
+    const int tid = team_tid<TEAM>(), V = R.V, nvec = V / N, mine = team_in_block<TEAM>();
+    const int words = bit_words<T, TEAM>(V);
+    unsigned* bits = bits_all + mine * words;
+    Entries& E = Es[mine];
+    constexpr int U = NV >= GROUP ? GROUP : NV > 0 ? NV : 1, Q = NV > 0 ? NV / U : 1;
+    Loaded<T, U> L[Q];
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) load_group<T, TEAM, U>(L[q], x, tid + q * U * TEAM, nvec);
+    }
+    if (Te.rest)
+        for (int i = tid; i < words; i += TEAM) bits[i] = 0;
+    EntryHead h;
+    if (tid < 64) {
+        h = load_entries<T>(E, Te, r, V, x, mk, R.c);
+        if (tid == 0) fars[mine] = h.far && Te.rest;
+    }
+    team_sync<TEAM>();
+    if (Te.rest) {
+        if (tid < 64)
+            for (int j = tid; j < Te.k; j += 64) set_bit(bits, E.id[j], 0, V);
+        team_sync<TEAM>();
+    }
+    const SkipBits<T> skip{bits, Te.rest != 0};
+    Sum a{-FAR, 0.f, 0.f};
+    float mx = -INFINITY;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            float f[U * N], gm = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int vi = tid + (q * U + u) * TEAM;
+                unpack<T>(L[q].v[u], f + u * N);
+                if (vi < nvec) {
+                    if constexpr (MASK) apply_mask<T>(mk + (long long)vi * N, f + u * N);
+                    skip(vi, f + u * N);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) gm = nmax(gm, f[u * N + i]);
+            }
+            mx = nmax(mx, gm);
+            sum_group<false, U * N>(a, f, gm, R.c);
+            __builtin_amdgcn_sched_barrier(0);  // one group unpacked at a time
+        }
+        const int i = nvec * N + tid;
+        if (nvec * N < V) {
+            float f[2] = {-INFINITY, -INFINITY};
+            if (i < V && (!MASK || mk[i]) && !skip.one(i)) f[0] = (float)x[i];
+            mx = nmax(mx, f[0]);
+            sum_group<false, 2>(a, f, f[0], R.c);
+        }
+    } else {
+        Best none{-INFINITY, 0};
+        row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip);
+    }
+    const Stat v = row_stat<T, TEAM>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
+    if (tid < 64) {
+        const Row o = finish_row(R, Te, E, h, v, O.row_loss + r);
+        if (tid == 0) {
+            rows[mine] = o;
+            if (O.stats) ((Row*)O.stats)[r] = o;
+        }
+    }
+    if (!O.dx) return;
+    team_sync<TEAM>();
+    if constexpr (NV > 0 && sizeof(T) == 2) {
+        // hides from the compiler that the packed logits are those already unpacked: it would keep the unpacked
+        // ones, twice the registers, over the reduction
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                asm volatile("" : "+v"(L[q].v[u].x), "+v"(L[q].v[u].y), "+v"(L[q].v[u].z), "+v"(L[q].v[u].w));
+    }
+    const Row o = rows[mine];
+    const float g = row_weight(R, O, r);
+    T* d = (T*)O.dx + r * (long long)V;
+    if (NV > 0 && o.wide == 0.f && o.so != 0.f) {
+        const float b = o.b * g / o.so;
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int vi = tid + (q * U + u) * TEAM;
+                if (vi >= nvec) continue;
+                float y[N];
+                unpack<T>(L[q].v[u], y);
+                if constexpr (MASK) apply_mask<T>(mk + (long long)vi * N, y);
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = ex2(__builtin_fmaf(y[i], R.c, -o.ro)) * b;
+                store16(d + (long long)vi * N, y);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        const int i = nvec * N + tid;
+        if (i < V) d[i] = (T)(!MASK || mk[i] ? ex2(__builtin_fmaf((float)x[i], R.c, -o.ro)) * b : 0.f);
+    } else {
+        write_outside<T, TEAM, MASK>(R, o, g, x, mk, d, V);
+    }
+    team_sync<TEAM>();
+    write_entries<T, TEAM>(R, Te, E, o, g, mk, d, 0, V);
+}
+
+// a part of a row of few rows: its statistics outside the entries
+template <class T, bool MASK>
+__global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, Split P) {
+    extern __shared__ unsigned bits[];
+    __shared__ Shared sh;
+    const long long r = block_row();
+    if (r >= R.rows) return;
+    const int tid = threadIdx.x, from = blockIdx.z * P.len, V = R.V - from < P.len ? R.V - from : P.len;
+    const T* x = row_ptr<T>(R, r) + from;
+    const uint8_t* mk = MASK ? mask_ptr(R, r) + from : nullptr;
+    if (Te.rest) {
+        for (int i = tid; i < bit_words<T, 256>(V); i += 256) bits[i] = 0;
+        int id = -1;
+        if (tid < Te.k) {
+            const long long o = r * Te.k + tid;
+            const long long i = Te.ids64 ? ((const long long*)Te.ids)[o] : ((const int*)Te.ids)[o];
+            const float f = Te.dtype == AZG_F32 ? ((const float*)Te.logp)[o]
+                            : Te.dtype == AZG_BF16 ? (float)((const bf16_t*)Te.logp)[o]
+                                                   : (float)((const f16_t*)Te.logp)[o];
+            if (i >= 0 && i < R.V && f != -INFINITY) id = (int)i;
+        }
+        __syncthreads();
+        set_bit(bits, id, from, V);
+        __syncthreads();
+    }
+    Sum a{-FAR, 0.f, 0.f};
+    float mx = -INFINITY;
+    Best none{-INFINITY, 0};
+    row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0});
+    a = team_sum<256>(a, sh.sum);
+    const bool plain = plain_sum(a);
+    const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
+    if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, 0.f, again);
+}
+
+// a row or a part of it of the gradient, from the row's statistics (stats) or from its parts (JOIN: then the first
+// part's block writes the row's loss and statistics as well)
+template <class T, int TEAM, bool MASK, bool JOIN>
+__global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Teacher Te, DistillOut O, Split P, int len) {
+    constexpr int TEAMS = block_of<TEAM> / TEAM;
+    __shared__ Shared sh;
+    __shared__ Entries Es[TEAMS];
+    __shared__ Row row;
+    __shared__ float4 joined;
+    const long long r = R.rows - 1 - team_row<TEAM>();
+    if (r < 0) return;
+    const int tid = team_tid<TEAM>(), from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
+    const T* x = row_ptr<T>(R, r);
+    const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
+    Entries& E = Es[team_in_block<TEAM>()];
+    EntryHead h;
+    if (tid < 64) h = load_entries<T>(E, Te, r, R.V, x, mk, R.c);
+    Row o;
+    if constexpr (JOIN) {
+        if (tid < 64) {
+            Sum a{-FAR, 0.f, 0.f};
+            bool again = Te.rest && h.far;
+            for (int i = tid; i < P.n; i += 64) {
+                const float4 p = P.part[r * P.n + i];
+                const float m = fmaxf(a.r, p.x);
+                const Sum b = move_sum(Sum{p.x, p.y, 0.f}, m);
+                a = move_sum(a, m);
+                a.s += b.s;
+                again |= p.w != 0.f;
+            }
+            a = team_sum<64>(a, nullptr);
+            again = __ballot(again) != 0;
+            if (tid == 0) joined = make_float4(a.s > 0.f ? a.r : 0.f, a.s, 0.f, again);
+        }
+        __syncthreads();
+        Stat v{joined.x, joined.y, 0.f, false};
+        if (joined.w != 0.f) {
+            const bool rest = Te.rest;
+            const int k = Te.k;
+            const Soft s = soft_pass<T, TEAM>(x, mk, R.V, R.c, sh.soft, [&](int i) {
+                for (int j = 0; rest && j < k; ++j)
+                    if (E.id[j] == i) return true;
+                return false;
+            });
+            v = Stat{s.m, s.s, 0.f, true};
+        }
+        if (tid < 64) {
+            const bool first = blockIdx.z == 0;
+            o = finish_row(R, Te, E, h, v, first ? O.row_loss + r : nullptr);
+            if (tid == 0) {
+                row = o;
+                if (O.stats && first) ((Row*)O.stats)[r] = o;
+            }
+        }
+        if (!O.dx) return;
+        __syncthreads();
+        o = row;
+    } else {
+        o = ((const Row*)O.stats)[r];
+    }
+    const float g = row_weight(R, O, r);
+    T* d = (T*)O.dx + r * (long long)R.V + from;
+    write_outside<T, TEAM, MASK>(R, o, g, x + from, MASK ? mk + from : nullptr, d, V);
+    team_sync<TEAM>();
+    write_entries<T, TEAM>(R, Te, E, o, g, MASK ? mk + from : nullptr, d, from, V);
 }
 
 // out = scale sum_r w_r loss_r in a fixed order, f64
@@ -517,10 +1312,16 @@ int launched() {
 int bad(const char* what) { return azg_host_fail(AZG_ERR_ARG, what); }
 
 template <class F>
-int by_type(int dtype, F f) {
+auto by_type(int dtype, F f) {
     if (dtype == AZG_F32) return f(float{});
     if (dtype == AZG_BF16) return f(bf16_t{});
     return f(f16_t{});
+}
+
+template <class F>
+int by_mask(const Rows& R, F f) {
+    if (R.mask) return f(std::true_type{});
+    return f(std::false_type{});
 }
 
 bool teacher_of(const azg_teacher* t, Teacher* Te) {
@@ -530,17 +1331,132 @@ bool teacher_of(const azg_teacher* t, Teacher* Te) {
     return true;
 }
 
+// Which team takes a row.  A wave: rows of up to 4 KB (a block would leave most of its threads idle).  A block:
+// longer ones.  Parts: rows longer than a block's LDS holds the maxima or bits of, and, where there are fewer rows
+// than would fill the chip, rows of more than 8192 elements, in parts of 4096 or more.
+constexpr int WAVE_BYTES = 4096, PART_MIN = 4096;
+template <class T>
+constexpr int BLOCK_MAX = sizeof(T) == 4 ? 65536 : 131072;
+
+template <class T>
+Split parts_of(const Rows& R) {
+    Split P{nullptr, nullptr, 1, R.V};
+    long long n = (R.V + BLOCK_MAX<T> - 1) / BLOCK_MAX<T>;
+    if (R.rows < 128 && R.V > 2 * PART_MIN) {
+        long long want = 512 / R.rows, most = R.V / PART_MIN;
+        if (want > most) want = most;
+        if (want > n) n = want;
+    }
+    if (n > 1) {
+        P.len = (int)(((R.V + n - 1) / n + 1023) / 1024 * 1024);
+        P.n = (R.V + P.len - 1) / P.len;
+    }
+    return P;
+}
+template <class T>
+bool by_wave(const Rows& R) { return (long long)R.V * (int)sizeof(T) <= WAVE_BYTES; }
+
+template <int TEAM>
+dim3 team_grid(long long rows, int z = 1) {
+    dim3 g = row_grid(TEAM == 64 ? (rows + 3) / 4 : rows);
+    g.z = (unsigned)z;
+    return g;
+}
+template <class T, int TEAM>
+unsigned gmax_bytes(int V) {
+    const int ng = (V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP);
+    return (unsigned)((ng + 1) * block_of<TEAM> * 4);
+}
+template <class T, int TEAM>
+unsigned bits_bytes(const Teacher& Te, int V) {
+    return Te.rest ? (unsigned)(bit_words<T, TEAM>(V) * 4 * (block_of<TEAM> / TEAM)) : 0;
+}
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+constexpr int BWD_LEN = 16384;  // elements of a row that a block of a gradient kernel takes
+
+template <class T, bool MASK>
+void distill_bwd(const Rows& R, const Teacher& Te, const DistillOut& O, hipStream_t st) {
+    const Split none{nullptr, nullptr, 0, 0};
+    if (by_wave<T>(R))
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 64, MASK, false>), team_grid<64>(R.rows), dim3(256), 0, st, R, Te, O,
+                           none, R.V);
+    else
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256, MASK, false>),
+                           team_grid<256>(R.rows, (R.V + BWD_LEN - 1) / BWD_LEN), dim3(256), 0, st, R, Te, O, none,
+                           BWD_LEN);
+}
+
+template <class T, int TEAM, bool MASK, int NV>
+void distill_rows(const Rows& R, const Teacher& Te, const DistillOut& O, hipStream_t st) {
+    hipLaunchKernelGGL((distill_rows_kernel<T, TEAM, MASK, NV>), team_grid<TEAM>(R.rows), dim3(block_of<TEAM>),
+                       (bits_bytes<T, TEAM>(Te, R.V)), st, R, Te, O);
+}
+
+template <class T, bool MASK>
+void distill_fwd(const Rows& R, const Teacher& Te, const DistillOut& O, Split P, float4* work, hipStream_t st) {
+    constexpr int N = VN<T>;
+    const int V = R.V;
+    if (P.n > 1) {
+        P.part = work;
+        hipLaunchKernelGGL((distill_part_kernel<T, MASK>), team_grid<256>(R.rows, P.n), dim3(256),
+                           (bits_bytes<T, 256>(Te, P.len)), st, R, Te, P);
+        hipLaunchKernelGGL((distill_bwd_kernel<T, 256, MASK, true>), team_grid<256>(R.rows, O.dx ? P.n : 1), dim3(256),
+                           0, st, R, Te, O, P, P.len);
+    } else if (!O.dx) {
+        if (by_wave<T>(R))
+            distill_rows<T, 64, MASK, 0>(R, Te, O, st);
+        else
+            distill_rows<T, 256, MASK, 0>(R, Te, O, st);
+    } else if (V <= 64 * N * 2) {
+        distill_rows<T, 64, MASK, 2>(R, Te, O, st);
+    } else if (V <= 64 * N * 8) {
+        distill_rows<T, 64, MASK, 8>(R, Te, O, st);
+    } else if (V <= 256 * N * 8) {
+        distill_rows<T, 256, MASK, 8>(R, Te, O, st);
+    } else if (V <= 256 * N * 16) {
+        distill_rows<T, 256, MASK, 16>(R, Te, O, st);
+    } else if (V <= 512 * N * 16) {
+        distill_rows<T, 512, MASK, 16>(R, Te, O, st);
+    } else {
+        distill_rows<T, 1024, MASK, 16>(R, Te, O, st);
+    }
+}
+
+template <class T, bool MASK, bool TOP>
+void logprobs_fwd(const Rows& R, const LogprobsOut& O, Split P, char* work, hipStream_t st) {
+    if (P.n > 1) {
+        P.part = (float4*)work;
+        P.keys = (unsigned long long*)(work + up16(R.rows * P.n * 16));
+        hipLaunchKernelGGL((logprobs_rows_kernel<T, 256, MASK, TOP, true>), team_grid<256>(R.rows, P.n), dim3(256),
+                           TOP ? (gmax_bytes<T, 256>(P.len)) : 0, st, R, O, P);
+        hipLaunchKernelGGL((logprobs_join_kernel<T, TOP>), team_grid<256>(R.rows), dim3(256), 0, st, R, O, P);
+    } else if (by_wave<T>(R) && (O.k <= 64 || R.V <= TopShare<64>::CANDS)) {
+        hipLaunchKernelGGL((logprobs_rows_kernel<T, 64, MASK, TOP, false>), team_grid<64>(R.rows), dim3(256),
+                           TOP ? (gmax_bytes<T, 64>(R.V)) : 0, st, R, O, P);
+    } else {
+        hipLaunchKernelGGL((logprobs_rows_kernel<T, 256, MASK, TOP, false>), team_grid<256>(R.rows), dim3(256),
+                           TOP ? (gmax_bytes<T, 256>(R.V)) : 0, st, R, O, P);
+    }
+}
+
 }  // namespace
 
 extern "C" int64_t azg_logprobs_work(const azg_logits* L, int32_t top) {
     Rows R;
     if (!rows_of(L, &R) || top < 0 || top > TOP_MAX) return bad("azg_logprobs_work: bad argument");
-    return 0;
+    return by_type(L->dtype, [&](auto z) -> int64_t {
+        const Split P = parts_of<decltype(z)>(R);
+        return P.n > 1 ? up16(R.rows * P.n * 16) + R.rows * P.n * top * 8 : 0;
+    });
 }
 extern "C" int64_t azg_distill_work(const azg_logits* L, int32_t) {
     Rows R;
     if (!rows_of(L, &R)) return bad("azg_distill_work: bad argument");
-    return 0;
+    return by_type(L->dtype, [&](auto z) -> int64_t {
+        const Split P = parts_of<decltype(z)>(R);
+        return P.n > 1 ? R.rows * P.n * 16 : 0;
+    });
 }
 
 extern "C" int azg_logprobs_fwd(const azg_logits* L, const void* actions, int32_t actions64, int32_t top, float* stats,
@@ -548,19 +1464,23 @@ extern "C" int azg_logprobs_fwd(const azg_logits* L, const void* actions, int32_
                                 int64_t work_bytes, void* stream) {
     Rows R;
     if (!rows_of(L, &R) || !entropy || !lse || (actions != nullptr) != (logp != nullptr) || top < 0 || top > TOP_MAX ||
-        (top > 0 && (!top_logp || !top_ids)) || work_bytes < azg_logprobs_work(L, top))
+        (top > 0 && (!top_logp || !top_ids)))
         return bad("azg_logprobs_fwd: bad argument");
-    hipStream_t st = (hipStream_t)stream;
-    return by_type(L->dtype, [&](auto z) {
+    const int64_t need = azg_logprobs_work(L, top);
+    if (need > 0 && (!work || work_bytes < need)) return bad("azg_logprobs_fwd: work is too small");
+    const LogprobsOut O{actions, actions64 != 0, top, stats, logp, entropy, lse, top_logp, (long long*)top_ids};
+    by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
-        if (top)
-            hipLaunchKernelGGL((logprobs_rows_kernel<T, true>), row_grid(L->rows), dim3(256), 0, st, R, actions,
-                               actions64, top, stats, logp, entropy, lse, top_logp, (long long*)top_ids);
-        else
-            hipLaunchKernelGGL((logprobs_rows_kernel<T, false>), row_grid(L->rows), dim3(256), 0, st, R, actions,
-                               actions64, top, stats, logp, entropy, lse, top_logp, (long long*)top_ids);
-        return launched();
+        return by_mask(R, [&](auto m) {
+            constexpr bool MASK = decltype(m)::value;
+            if (top)
+                logprobs_fwd<T, MASK, true>(R, O, parts_of<T>(R), (char*)work, (hipStream_t)stream);
+            else
+                logprobs_fwd<T, MASK, false>(R, O, parts_of<T>(R), (char*)work, (hipStream_t)stream);
+            return 0;
+        });
     });
+    return launched();
 }
 
 extern "C" int azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_t actions64, const float* stats,
@@ -569,13 +1489,24 @@ extern "C" int azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_
                                 void* stream) {
     Rows R;
     if (!rows_of(L, &R) || !stats || !dx || (g_logp && !actions)) return bad("azg_logprobs_bwd: bad argument");
-    return by_type(L->dtype, [&](auto z) {
+    by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
-        hipLaunchKernelGGL((logprobs_bwd_kernel<T>), row_grid(L->rows), dim3(256), 0, (hipStream_t)stream, R,
-                           actions, actions64, stats, g_logp, (long long)g_logp_stride, g_entropy,
-                           (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx);
-        return launched();
+        return by_mask(R, [&](auto m) {
+            constexpr bool MASK = decltype(m)::value;
+            if (by_wave<T>(R))
+                hipLaunchKernelGGL((logprobs_bwd_kernel<T, 64, MASK>), team_grid<64>(R.rows), dim3(256), 0,
+                                   (hipStream_t)stream, R, actions, actions64, stats, g_logp, (long long)g_logp_stride,
+                                   g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx, R.V);
+            else
+                hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, MASK>),
+                                   team_grid<256>(R.rows, (R.V + BWD_LEN - 1) / BWD_LEN), dim3(256), 0,
+                                   (hipStream_t)stream, R, actions, actions64, stats, g_logp, (long long)g_logp_stride,
+                                   g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx,
+                                   BWD_LEN);
+            return 0;
+        });
     });
+    return launched();
 }
 
 extern "C" int azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float* stats, float* row_loss,
@@ -583,21 +1514,22 @@ extern "C" int azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float*
                                void* work, int64_t work_bytes, void* stream) {
     Rows R;
     Teacher Te;
-    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !row_loss || (dx && !stats) ||
-        work_bytes < azg_distill_work(L, dx != nullptr))
-        return bad("azg_distill_fwd: bad argument");
+    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !row_loss) return bad("azg_distill_fwd: bad argument");
+    const int64_t need = azg_distill_work(L, dx != nullptr);
+    if (need > 0 && (!work || work_bytes < need)) return bad("azg_distill_fwd: work is too small");
     hipStream_t st = (hipStream_t)stream;
-    return by_type(L->dtype, [&](auto z) {
+    const DistillOut O{stats, row_loss, weight, (long long)weight_stride, scale, dx};
+    by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
-        hipLaunchKernelGGL((distill_rows_kernel<T>), row_grid(L->rows), dim3(256), 0, st, R, Te, stats, row_loss);
-        if (dx)
-            hipLaunchKernelGGL((distill_bwd_kernel<T>), row_grid(L->rows), dim3(256), 0, st, R, Te, stats, weight,
-                               (long long)weight_stride, scale, (T*)dx);
-        if (total)
-            hipLaunchKernelGGL(loss_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, weight,
-                               (long long)weight_stride, scale, (long long)L->rows, total);
-        return launched();
+        return by_mask(R, [&](auto m) {
+            distill_fwd<T, decltype(m)::value>(R, Te, O, parts_of<T>(R), (float4*)work, st);
+            return 0;
+        });
     });
+    if (total)
+        hipLaunchKernelGGL(loss_total_kernel, dim3(1), dim3(1024), 0, st, row_loss, weight, (long long)weight_stride,
+                           scale, (long long)L->rows, total);
+    return launched();
 }
 
 extern "C" int azg_distill_bwd(const azg_logits* L, const azg_teacher* t, const float* stats, const float* weight,
@@ -605,10 +1537,13 @@ extern "C" int azg_distill_bwd(const azg_logits* L, const azg_teacher* t, const 
     Rows R;
     Teacher Te;
     if (!rows_of(L, &R) || !teacher_of(t, &Te) || !stats || !dx) return bad("azg_distill_bwd: bad argument");
-    return by_type(L->dtype, [&](auto z) {
+    const DistillOut O{const_cast<float*>(stats), nullptr, weight, (long long)weight_stride, scale, dx};
+    by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
-        hipLaunchKernelGGL((distill_bwd_kernel<T>), row_grid(L->rows), dim3(256), 0, (hipStream_t)stream, R, Te,
-                           stats, weight, (long long)weight_stride, scale, (T*)dx);
-        return launched();
+        return by_mask(R, [&](auto m) {
+            distill_bwd<T, decltype(m)::value>(R, Te, O, (hipStream_t)stream);
+            return 0;
+        });
     });
+    return launched();
 }

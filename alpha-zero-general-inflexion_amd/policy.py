@@ -26,7 +26,7 @@ import torch
 from . import _lib
 
 TOP_MAX = 128      # azg.h AZG_POLICY_TOP_MAX
-VOCAB_MAX = 1 << 30
+VOCAB_MAX = 1 << 29
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum azg_dtype
 
 ActionLogprobs = namedtuple("ActionLogprobs", "logp entropy lse top_logp top_ids")
@@ -257,7 +257,7 @@ def _distill(logits, mask, t, t_logp, t_ids, rest, weight, scale, want_stats, wa
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     total = torch.empty((), dtype=torch.float32, device=dev) if want_total else None
     dx = torch.empty(shape, dtype=logits.dtype, device=dev) if want_grad else None
-    stats = torch.empty((n, 8), dtype=torch.float32, device=dev) if want_stats or want_grad else None
+    stats = torch.empty((n, 8), dtype=torch.float32, device=dev) if want_stats else None
     if n:
         w, ws = _spread(weight)
         lib = _lib.lib()

@@ -486,13 +486,13 @@ int  azg_train_loss_bwd(const float* x3, int32_t ld3, const float* z4, int32_t l
  * azg_distill_fwd: row_loss [rows] = KL(teacher || student), 0 for a row without an entry or without a
  *   legal action; total (may be null) = scale sum_r weight_r row_loss_r (weight null: 1; a stride of 0
  *   repeats one value; f64, fixed order); dx (may be null) = the gradient of that sum.  stats [rows][8]
- *   (16-B aligned, may be null without dx) is what azg_distill_bwd needs, which writes dx = the gradient of
+ *   (16-B aligned, may be null) is what azg_distill_bwd needs, which writes dx = the gradient of
  *   scale sum_r weight_r row_loss_r.
  * work: azg_logprobs_work / azg_distill_work bytes of scratch (16-B aligned; 0: may be null; -1: a bad
  *   argument), in use until the call's kernels end.  1 <= rows <= AZG_POLICY_ROWS_MAX, 1 <= vocab <= AZG_POLICY_VOCAB_MAX. */
 #define AZG_POLICY_TOP_MAX 128
 #define AZG_POLICY_ROWS_MAX (1LL << 35)
-#define AZG_POLICY_VOCAB_MAX (1LL << 30)
+#define AZG_POLICY_VOCAB_MAX (1LL << 29)
 enum azg_dtype { AZG_F32 = 0, AZG_BF16 = 1, AZG_F16 = 2 };
 typedef struct azg_logits {
     const void* x;

@@ -109,4 +109,9 @@ def test_c_entries_refuse():
         u = _lib.Teacher(*d.values())
         assert L.azg_distill_fwd(g, u, p, p, None, 0, 1.0, None, p, None, 0, None) == -1
         assert L.azg_distill_bwd(g, u, p, None, 0, 1.0, p, None) == -1
-    assert L.azg_distill_fwd(g, t, None, p, None, 0, 1.0, None, p, None, 0, None) == -1  # a gradient needs stats
+    # rows in parts need their scratch memory
+    g = logits(vocab=2 ** 20)
+    assert L.azg_logprobs_work(g, 8) > 0 and L.azg_distill_work(g, 1) > 0
+    assert L.azg_logprobs_fwd(g, None, 0, 0, None, None, p, p, None, None, None, 0, None) == -1
+    assert L.azg_distill_fwd(g, t, p, p, None, 0, 1.0, None, p, p, 16, None) == -1
+    assert b"work" in L.azg_last_error()
