@@ -45,14 +45,18 @@ struct Rows {
     float invT;  // 1 / T
 };
 
+// (rows at one stride, the usual case, are spared the 64-bit division)
+__device__ __forceinline__ long long row_at(const Rows& R, long long r, long long so, long long si) {
+    if (R.inner >= R.rows) return r * si;
+    const long long o = r / R.inner;
+    return o * so + (r - o * R.inner) * si;
+}
 template <class T>
 __device__ __forceinline__ const T* row_ptr(const Rows& R, long long r) {
-    const long long o = r / R.inner, i = r - o * R.inner;
-    return (const T*)R.x + o * R.so + i * R.si;
+    return (const T*)R.x + row_at(R, r, R.so, R.si);
 }
 __device__ __forceinline__ const uint8_t* mask_ptr(const Rows& R, long long r) {
-    const long long o = r / R.inner, i = r - o * R.inner;
-    return R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
+    return R.mask ? R.mask + row_at(R, r, R.mo, R.mi) : nullptr;
 }
 
 // rows over the grid's x and y (a dimension holds fewer than 2^32 threads)
@@ -125,17 +129,25 @@ __device__ __forceinline__ int team_in_block() { return TEAM == 64 ? threadIdx.x
 template <int TEAM>
 __device__ __forceinline__ long long team_row() { return TEAM == 64 ? block_row() * 4 + (threadIdx.x >> 6) : block_row(); }
 
-// ---- vectors of 16 bytes (a row may start at any element: the loads need no more than its alignment) ----
+// ---- vectors of 16 bytes ------------------------------------------------------------------------------
+// A row may start at any element and so may its vectors (the loads need no more than the element's alignment; vectors
+// from the first 16-byte boundary on measured no faster: 76.8 us against 76.2, 4092 x 50001 bf16); the elements
+// behind the last whole one are taken one a thread.
 template <class T>
 constexpr int VN = 16 / (int)sizeof(T);
 template <class T>
 constexpr unsigned MINF_BITS = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, f16_t> ? 0xFC00FC00u : 0xFF80FF80u;
 
-template <class T>
+// NT: without a place in the caches, for what is not read again (6.4 TB/s against 5.6, 4096 x 65536 f16)
+template <bool NT, class T>
 __device__ __forceinline__ uint4 load16(const T* p) {
-    uint4 v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    W w;
+    if constexpr (NT)
+        w = __builtin_nontemporal_load((const W*)p);
+    else
+        w = *(const W*)p;
+    return make_uint4(w.x, w.y, w.z, w.w);
 }
 template <class T>
 __device__ __forceinline__ void unpack(const uint4& v, float* f) {
@@ -153,12 +165,18 @@ __device__ __forceinline__ void unpack(const uint4& v, float* f) {
         }
     }
 }
-template <class T>
+template <bool NT, class T>
 __device__ __forceinline__ void store16(T* p, const float* f) {
+    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     T t[VN<T>];
 #pragma unroll
     for (int i = 0; i < VN<T>; ++i) t[i] = (T)f[i];  // round to nearest even
-    __builtin_memcpy(p, t, 16);
+    W w;
+    __builtin_memcpy(&w, t, 16);
+    if constexpr (NT)
+        __builtin_nontemporal_store(w, (W*)p);
+    else
+        *(W*)p = w;
 }
 // illegal actions of a vector -> -inf
 template <class T>
@@ -330,18 +348,26 @@ template <class T, int U>
 struct Loaded {
     uint4 v[U];
 };
-template <class T, int TEAM, int U>
+template <class T, int TEAM, int U, bool NT>
 __device__ __forceinline__ void load_group(Loaded<T, U>& L, const T* x, int vi, int nvec) {
     if (vi - team_tid<TEAM>() + TEAM * U <= nvec) {  // the whole team's
 #pragma unroll
-        for (int u = 0; u < U; ++u) L.v[u] = load16(x + (long long)(vi + u * TEAM) * VN<T>);
+        for (int u = 0; u < U; ++u) L.v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * VN<T>);
     } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             L.v[u] = make_uint4(MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>);
-            if (vi + u * TEAM < nvec) L.v[u] = load16(x + (long long)(vi + u * TEAM) * VN<T>);
+            if (vi + u * TEAM < nvec) L.v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * VN<T>);
         }
     }
+}
+
+// Hides from the compiler what these registers hold: it would unpack all groups at once, and keep the unpacked
+// logits (twice the registers) from one use to the next.
+template <class T, int U>
+__device__ __forceinline__ void opaque(Loaded<T, U>& L) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) asm volatile("" : "+v"(L.v[u].x), "+v"(L.v[u].y), "+v"(L.v[u].z), "+v"(L.v[u].w));
 }
 
 // what the top alternatives need of a pass: each thread's best vector and the maximum of each of its groups (LDS)
@@ -357,21 +383,21 @@ struct NoEdit {
     __device__ __forceinline__ bool one(int) const { return false; }
 };
 
-template <class T, int TEAM, bool MASK, bool ENT, bool TOP, class Edit>
-__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx, Best& best,
-                                         float* gmax, const Edit& edit) {
+template <class T, int TEAM, bool MASK, bool ENT, bool TOP, bool NT, class Edit>
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx,
+                                         Best& best, float* gmax, const Edit& edit) {
     constexpr int N = VN<T>;
     const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
     int g = 0;
     for (int vi = tid; vi - tid < nvec; vi += step, ++g) {
         Loaded<T, GROUP> L;
-        load_group<T, TEAM, GROUP>(L, x, vi, nvec);
+        load_group<T, TEAM, GROUP, NT>(L, x, vi, nvec);
         float f[GROUP * N], vm[GROUP];
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
             unpack<T>(L.v[u], f + u * N);
             if constexpr (MASK)
-                if (vi + u * TEAM < nvec) apply_mask<T>(mk + (long long)(vi + u * TEAM) * N, f + u * N);
+                if (vi + u * TEAM < nvec) apply_mask<T>(mk + (vi + u * TEAM) * N, f + u * N);
             edit(vi + u * TEAM, f + u * N);
             float m = f[u * N];
 #pragma unroll
@@ -390,15 +416,23 @@ __device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, f
         if constexpr (TOP) gmax[g * TEAM + tid] = gm;
         sum_group<ENT, GROUP * N>(a, f, gm, c);
     }
-    const int rest = V - nvec * N, i = nvec * N + tid;  // the last, incomplete vector, an element a thread
     float f[2] = {-INFINITY, -INFINITY};
-    if (tid < rest && (!MASK || mk[i]) && !edit.one(i)) f[0] = (float)x[i];
+    const int i = nvec * N + tid;
+    if (i < V && (!MASK || mk[i]) && !edit.one(i)) f[0] = (float)x[i];
     if constexpr (TOP) {
         gmax[g * TEAM + tid] = f[0];
         if (f[0] > best.v) best = Best{f[0], i};
     }
     mx = nmax(mx, f[0]);
-    if (rest) sum_group<ENT, 2>(a, f, f[0], c);
+    if (nvec * N < V) sum_group<ENT, 2>(a, f, f[0], c);
+}
+template <class T, int TEAM, bool MASK, bool ENT, bool TOP, class Edit>
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx,
+                                         Best& best, float* gmax, const Edit& edit, bool nt) {
+    if (nt)  // the same for the whole team
+        row_pass<T, TEAM, MASK, ENT, TOP, true>(x, mk, V, c, a, mx, best, gmax, edit);
+    else
+        row_pass<T, TEAM, MASK, ENT, TOP, false>(x, mk, V, c, a, mx, best, gmax, edit);
 }
 
 // the row again, an element at a time, for what Sum does not hold
@@ -576,7 +610,7 @@ __device__ int top_select(const T* x, const uint8_t* mk, int V, int k, bool plai
                     const int vi = (g * GROUP + u) * TEAM + t;
                     i0 = vi * N;
                     if (vi < nvec) {
-                        unpack<T>(load16(x + i0), f);
+                        unpack<T>(load16<false>(x + i0), f);
                         if constexpr (MASK) apply_mask<T>(mk + i0, f);
                         n = N;
                     }
@@ -618,6 +652,7 @@ struct LogprobsOut {
     int act64, k;
     float *stats, *logp, *entropy, *lse, *top_logp;
     long long* top_ids;
+    long long keep;  // rows from here on are left in the caches for the backward pass
 };
 
 // a row's given action: its index is read ahead of the pass, its logit (by then cached) after it
@@ -669,14 +704,13 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
         x += from;
         if constexpr (MASK) mk += from;
     }
-    const int ng = (V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP);
-    float* gmax = gmax_all + team_in_block<TEAM>() * (ng + 1) * TEAM;
+    float* gmax = gmax_all + team_in_block<TEAM>() * ((V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP) + 1) * TEAM;
     long long act = -1;
     if constexpr (!PART) act = action_of(O, r);
     Sum a{-FAR, 0.f, 0.f};
     float mx = -INFINITY;
     Best best{-INFINITY, 0};
-    row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{});
+    row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{}, r < O.keep);
     Stat st;
     float l2 = 0.f;
     if constexpr (PART) {
@@ -766,13 +800,13 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
 
 // Elementwise over a row or a part of it: f(x, legal) for each element, vectors of 16 bytes.  Rows are taken from
 // the last to the first: what a forward pass read last may still be in the Infinity Cache.
-template <class T, int TEAM, bool MASK, class F>
+template <class T, int TEAM, bool MASK, bool NT, class F>
 __device__ __forceinline__ void map_row(const T* x, const uint8_t* mk, T* d, int V, F f) {
     constexpr int N = VN<T>;
     const int tid = team_tid<TEAM>(), nvec = V / N;
     for (int vi = tid; vi - tid < nvec; vi += TEAM * GROUP) {
         Loaded<T, GROUP> L;
-        load_group<T, TEAM, GROUP>(L, x, vi, nvec);
+        load_group<T, TEAM, GROUP, true>(L, x, vi, nvec);
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
             const int i0 = (vi + u * TEAM) * N;
@@ -788,11 +822,20 @@ __device__ __forceinline__ void map_row(const T* x, const uint8_t* mk, T* d, int
 #pragma unroll
                 for (int i = 0; i < N; ++i) y[i] = f(y[i], i0 + i);
             }
-            store16(d + i0, y);
+            store16<NT>(d + i0, y);
         }
     }
     const int i = nvec * N + tid;
     if (i < V) d[i] = (T)(!MASK || mk[i] ? f((float)x[i], i) : 0.f);
+}
+
+template <class T, int TEAM, bool MASK, class F>
+__device__ __forceinline__ void map_row(const T* x, const uint8_t* mk, T* d, int V, bool nt, F f) {
+    // one loop or the other: within one the compiler joins the two kinds of store, and loses the hint
+    if (nt)
+        map_row<T, TEAM, MASK, true>(x, mk, d, V, f);
+    else
+        map_row<T, TEAM, MASK, false>(x, mk, d, V, f);
 }
 
 template <class T, int TEAM, bool MASK>
@@ -800,7 +843,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, co
                                                            const float* __restrict__ stats, const float* gl,
                                                            long long gl_s, const float* ge, long long ge_s,
                                                            const float* gz, long long gz_s, T* __restrict__ dx,
-                                                           int len) {
+                                                           int len, bool nt) {
     const long long r = R.rows - 1 - team_row<TEAM>();
     if (r < 0) return;
     const int from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
@@ -818,14 +861,14 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, co
     T* d = dx + r * (long long)R.V + from;
     const int at = given ? (int)(a - from) : -1;  // outside this part: no element's index
     if (s == 0.f) {  // no legal action
-        map_row<T, TEAM, false>(x, mk, d, V, [](float, int) { return 0.f; });
+        map_row<T, TEAM, false>(x, mk, d, V, nt, [](float, int) { return 0.f; });
     } else if (st.w != 0.f) {
-        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int i) {
+        map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int i) {
             const float u = nmax((y - ref) * R.c, -1000.f);
             return ex2(u) * (c0 - c1 * u) + (i == at ? ga : 0.f);
         });
     } else {
-        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int i) {
+        map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int i) {
             const float u = nmax(__builtin_fmaf(y, R.c, -ref), -1000.f);
             const float g = ex2(u) * __builtin_fmaf(-c1, u, c0);
             return i == at ? g + ga : g;
@@ -848,149 +891,183 @@ struct Entries {
     bool first[TOP_MAX];
 };
 struct EntryHead {
+    double Q;  // sum q
     float tm, qs;
     bool any, far;  // far: a student's logit that Sum does not hold
 };
-
-// by one wave, an entry or two a lane
-template <class T>
-__device__ __forceinline__ EntryHead load_entries(Entries& E, const Teacher& Te, long long r, int V, const T* x,
-                                                  const uint8_t* mk, float c) {
-    const int lane = threadIdx.x & 63;
-    float tm = -INFINITY;
-    float t[2];
+struct EntryRegs {  // as loaded, an entry or two a lane
     int id[2];
-    bool far = false;
+    float t[2], x[2];
+    bool legal[2];
+};
+
+// by one wave; nothing here waits for the last loads: what a team loads of the row comes behind them
+template <class T>
+__device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long r, int V, const T* x,
+                                                   const uint8_t* mk) {
+    const int lane = threadIdx.x & 63;
+    EntryRegs e;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
-        t[u] = -INFINITY;
-        id[u] = -1;
+        e.t[u] = -INFINITY;
+        e.id[u] = -1;
         if (j < Te.k) {
             const long long o = r * Te.k + j;
             const long long i = Te.ids64 ? ((const long long*)Te.ids)[o] : ((const int*)Te.ids)[o];
-            const float f = Te.dtype == AZG_F32 ? ((const float*)Te.logp)[o]
-                            : Te.dtype == AZG_BF16 ? (float)((const bf16_t*)Te.logp)[o]
-                                                   : (float)((const f16_t*)Te.logp)[o];
-            if (i >= 0 && i < V && f != -INFINITY) {
-                id[u] = (int)i;
-                t[u] = f;
-            }
-            float xj = -INFINITY;
-            if (id[u] >= 0 && (!mk || mk[id[u]])) xj = (float)x[id[u]];
-            E.id[j] = id[u];
-            E.t[j] = t[u];
-            E.x[j] = xj;
-            far |= xj != -INFINITY && !(fabsf(xj * c) < FAR);
+            e.id[u] = i >= 0 && i < V ? (int)i : -1;
+            e.t[u] = Te.dtype == AZG_F32 ? ((const float*)Te.logp)[o]
+                     : Te.dtype == AZG_BF16 ? (float)((const bf16_t*)Te.logp)[o]
+                                            : (float)((const f16_t*)Te.logp)[o];
         }
-        tm = nmax(tm, t[u]);
     }
-    tm = wave_max(tm);
-    const bool any = tm != -INFINITY;
-    if (Te.rest || !any) tm = 0.f;
-    float q[2], qs = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        q[u] = id[u] >= 0 ? expf(t[u] - tm) : 0.f;
-        qs += q[u];
+        const int i = e.id[u] < 0 ? 0 : e.id[u];
+        e.x[u] = (float)x[i];
+        e.legal[u] = !mk || mk[i];
     }
-    qs = wave_sum(qs);
-    const float iq = Te.rest || !any ? 1.f : 1.f / qs;
-    team_sync<64>();
-    bool dup[2] = {false, false};
-    if (Te.rest)
-        for (int i = 0; i + 1 < Te.k; ++i) {
-            const int e = E.id[i];
-            dup[0] |= i < lane && e == id[0];
-            dup[1] |= i < lane + 64 && e == id[1];
-        }
+    return e;
+}
+
+template <class T>
+__device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e, const Teacher& Te, float c) {
+    const int lane = threadIdx.x & 63;
+    EntryHead h;
+    int id[2];
+    bool far = false;
+    h.tm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        id[u] = e.t[u] == -INFINITY ? -1 : e.id[u];
+        if (id[u] >= 0) h.tm = nmax(h.tm, e.t[u]);
+    }
+    h.tm = wave_max(h.tm);
+    h.any = h.tm != -INFINITY;
+    if (Te.rest || !h.any) h.tm = 0.f;
+    float q[2];
+    h.qs = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        q[u] = id[u] >= 0 ? expf(e.t[u] - h.tm) : 0.f;
+        h.qs += q[u];
+    }
+    h.qs = wave_sum(h.qs);
+    const float iq = Te.rest || !h.any ? 1.f : 1.f / h.qs;
+    h.Q = 0.0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
+        q[u] *= iq;
+        h.Q += q[u];
         if (j < Te.k) {
-            E.q[j] = q[u] * iq;
-            E.first[j] = !dup[u];
+            const float xj = id[u] >= 0 && e.legal[u] ? e.x[u] : -INFINITY;
+            far |= xj != -INFINITY && !(fabsf(xj * c) < FAR);
+            E.id[j] = id[u];
+            E.t[j] = e.t[u];
+            E.x[j] = xj;
+            E.q[j] = q[u];
+            E.first[j] = true;
         }
     }
+    h.Q = wave_sum(h.Q);
+    h.far = __ballot(far) != 0;
     team_sync<64>();
-    return EntryHead{tm, qs, any, __ballot(far) != 0};
+    return h;
+}
+
+// which entries repeat an earlier one's id; true if any does
+__device__ __forceinline__ bool find_repeats(Entries& E, int k) {
+    const int lane = threadIdx.x & 63;
+    const int id0 = lane < k ? E.id[lane] : -1, id1 = lane + 64 < k ? E.id[lane + 64] : -1;
+    bool d0 = false, d1 = false;
+#pragma unroll 8
+    for (int i = 0; i + 1 < k; ++i) {
+        const int e = E.id[i];
+        d0 |= i < lane && e == id0;
+        d1 |= i < lane + 64 && e == id1;
+    }
+    d0 &= id0 >= 0;
+    d1 &= id1 >= 0;
+    if (d0) E.first[lane] = false;
+    if (d1) E.first[lane + 64] = false;
+    team_sync<64>();
+    return __ballot(d0 || d1) != 0;
 }
 
 struct Row {  // what the gradient needs of a row: p(x, ref, s) = 2^u(x, ref) / s
     float ro, so, b;  // dx = b p(x, ro, so) w / T, but
     float ra, sa, a;  // dx = (a p(x, ra, sa) - q) w / T at the entries
-    float wide, pad;
+    float wide, repeats;
 };
 
-// one row's loss and coefficients, by one wave, from the student's statistics over all legal actions outside the
-// entries (rest) or over all (else)
-__device__ __forceinline__ Row finish_row(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
-                                          const Stat& v, float* row_loss) {
+// a row's coefficients, by one wave, from the student's statistics v over all legal actions outside the entries
+// (rest) or over all (else)
+__device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
+                                                const Stat& v, bool repeats) {
     const int lane = threadIdx.x & 63;
-    float xj[2];
-    bool ok[2];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int j = lane + 64 * u;
-        ok[u] = j < Te.k && E.id[j] >= 0;
-        xj[u] = ok[u] ? E.x[j] : -INFINITY;
-        mx = nmax(mx, xj[u]);
-    }
     Stat all = v;
+    float po = 1.f;  // the student's mass outside the entries
     if (Te.rest) {
+        float xj[2], mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int j = lane + 64 * u;
+            xj[u] = j < Te.k && E.first[j] ? E.x[j] : -INFINITY;
+            mx = nmax(mx, xj[u]);
+        }
         mx = wave_max(mx);
         Stat e{0.f, 0.f, 0.f, v.wide};
         if (mx != -INFINITY) {
             e.ref = v.wide ? mx : rintf(mx * R.c);
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (ok[u] && E.first[lane + 64 * u]) e.s += ex2(u_of(xj[u], e.ref, v.wide, R.c));
-            e.s = wave_sum(e.s);
+            e.s = wave_sum(ex2(u_of(xj[0], e.ref, v.wide, R.c)) + ex2(u_of(xj[1], e.ref, v.wide, R.c)));
         }
+        po = v.s != 0.f ? 1.f : 0.f;
         if (e.s != 0.f && v.s != 0.f) {
             all.ref = nmax(e.ref, v.ref);
-            const float de = v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref;
-            const float dv = v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref;
-            all.s = e.s * ex2(de) + v.s * ex2(dv);
+            const float se = e.s * ex2(v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref);
+            const float sv = v.s * ex2(v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref);
+            all.s = se + sv;
+            po = sv / all.s;
         } else if (e.s != 0.f) {
             all = e;
         }
     }
+    double S = h.Q, qr = 0.0;
+    if (Te.rest && v.s != 0.f) {
+        qr = 1.0 - h.Q;
+        if (qr < 0.0) qr = 0.0;
+        S += qr;
+    }
+    if (!h.any || all.s == 0.f) S = 0.0, qr = 0.0;
+    return Row{v.ref, v.s, (float)(S * (double)po - qr), all.ref, all.s, (float)S, v.wide ? 1.f : 0.f,
+               repeats ? 1.f : 0.f};
+}
+
+// the row's loss, by one wave, its terms in f64
+__device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
+                                        const Row& o) {
+    if (!h.any || o.sa == 0.f) return 0.f;
+    const int lane = threadIdx.x & 63;
+    const bool wide = o.wide != 0.f;
     const double cd = R.c, ln2 = 0.69314718055994530942;
-    const double lns = ln_f64(all.s), lnq = Te.rest ? 0.0 : ln_f64(h.qs);
-    double loss = 0.0, Q = 0.0;
+    const double lns = ln_f64(o.sa), lnq = Te.rest ? 0.0 : ln_f64(h.qs);
+    double loss = 0.0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        if (!ok[u]) continue;
         const int j = lane + 64 * u;
+        if (j >= Te.k || E.id[j] < 0) continue;
         const double q = E.q[j];
-        Q += q;
         const double lq = ((double)E.t[j] - (double)h.tm) - lnq;
-        const double uj = v.wide ? ((double)xj[u] - (double)all.ref) * cd : (double)xj[u] * cd - (double)all.ref;
-        const double lp = uj * ln2 - lns;
-        if (q > 0.0 || q != q) loss += q * (lq - lp);
+        const double uj = wide ? ((double)E.x[j] - (double)o.ra) * cd : (double)E.x[j] * cd - (double)o.ra;
+        if (q > 0.0 || q != q) loss += q * (lq - (uj * ln2 - lns));
     }
     loss = wave_sum(loss);
-    Q = wave_sum(Q);
-    double S = Q, pr = 1.0, qr = 0.0;
-    if (Te.rest) {
-        pr = 0.0;
-        if (v.s != 0.f) {
-            const double d = v.wide ? ((double)v.ref - (double)all.ref) * cd : (double)v.ref - (double)all.ref;
-            const double lpr = d * ln2 + ln_f64(v.s) - lns;
-            const double y = lpr * 1.4426950408889634074, yi = rint(y);
-            pr = (double)__builtin_amdgcn_ldexpf(ex2((float)(y - yi)), (int)fmax(yi, -4096.0));
-            if (lpr != lpr) pr = lpr;
-            qr = 1.0 - Q;
-            if (qr < 0.0) qr = 0.0;
-            if (qr != 0.0) loss += qr * (ln_f64((float)qr) - lpr);
-            S += qr;
-        }
+    if (Te.rest && o.so != 0.f) {
+        const double qr = 1.0 - h.Q, d = wide ? ((double)o.ro - (double)o.ra) * cd : (double)o.ro - (double)o.ra;
+        if (!(qr <= 0.0)) loss += qr * (ln_f64((float)qr) - (d * ln2 + ln_f64(o.so) - lns));
     }
-    if (!h.any || all.s == 0.f) loss = 0.0, S = 0.0, qr = 0.0;
-    if (lane == 0 && row_loss) *row_loss = (float)loss;
-    return Row{v.ref, v.s, (float)(S * pr - qr), all.ref, all.s, (float)S, v.wide ? 1.f : 0.f, 0.f};
+    return (float)loss;
 }
 
 // the entries of a row as bits, an element each: what a pass leaves out
@@ -1010,14 +1087,14 @@ struct SkipBits {
     }
     __device__ __forceinline__ bool one(int i) const { return on && (bits[i >> 5] >> (i & 31) & 1); }
 };
-// words of the bitmap: whole groups of vectors may be looked up past the row's end
-template <class T, int TEAM>
+// words of the bitmap: whole groups of vectors (NV of them) are looked up, also past the row's end
+template <class T, int TEAM, int NV = 0>
 __host__ __device__ constexpr int bit_words(int V) {
-    return (V / VN<T> / (TEAM * GROUP) + 1) * TEAM * GROUP * VN<T> / 32 + 1;
+    return (NV > 0 ? TEAM * NV : (V / VN<T> / (TEAM * GROUP) + 1) * TEAM * GROUP) * VN<T> / 32 + 1;
 }
-__device__ __forceinline__ void set_bit(unsigned* bits, int id, int from, int V) {
+__device__ __forceinline__ bool set_bit(unsigned* bits, int id, int from, int V) {  // was it set?
     const int i = id - from;
-    if (id >= 0 && i >= 0 && i < V) atomicOr(&bits[i >> 5], 1u << (i & 31));
+    return id >= 0 && i >= 0 && i < V && (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1);
 }
 
 // the entries' elements of a row (or a part of it), after all its elements
@@ -1027,8 +1104,11 @@ __device__ __forceinline__ void write_entries(const Rows& R, const Teacher& Te, 
     for (int j = team_tid<TEAM>(); j < Te.k; j += TEAM) {
         const int id = E.id[j], i = id - from;
         if (id < 0 || i < 0 || i >= V || (mk && !mk[i])) continue;
-        float q = 0.f;  // the same index twice: its entries' probabilities add
-        for (int e = 0; e < Te.k; ++e) q += E.id[e] == id ? E.q[e] : 0.f;
+        float q = E.q[j];
+        if (o.repeats != 0.f) {  // the same index twice: its entries' probabilities add
+            q = 0.f;
+            for (int e = 0; e < Te.k; ++e) q += E.id[e] == id ? E.q[e] : 0.f;
+        }
         const float p = ex2(u_of(E.x[j], o.ra, o.wide != 0.f, R.c)) * (o.a / o.sa);
         d[i] = (T)(o.a == 0.f ? 0.f : (p - q) * g);  // a = 0: a row without a legal action
     }
@@ -1036,14 +1116,14 @@ __device__ __forceinline__ void write_entries(const Rows& R, const Teacher& Te, 
 
 template <class T, int TEAM, bool MASK>
 __device__ __forceinline__ void write_outside(const Rows& R, const Row& o, float g, const T* x, const uint8_t* mk, T* d,
-                                              int V) {
+                                              int V, bool nt) {
     const float b = o.so == 0.f ? 0.f : o.b * g / o.so;
     if (o.so == 0.f)
-        map_row<T, TEAM, false>(x, mk, d, V, [](float, int) { return 0.f; });
+        map_row<T, TEAM, false>(x, mk, d, V, nt, [](float, int) { return 0.f; });
     else if (o.wide != 0.f)
-        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int) { return ex2((y - o.ro) * R.c) * b; });
+        map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int) { return ex2((y - o.ro) * R.c) * b; });
     else
-        map_row<T, TEAM, MASK>(x, mk, d, V, [&](float y, int) { return ex2(__builtin_fmaf(y, R.c, -o.ro)) * b; });
+        map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int) { return ex2(__builtin_fmaf(y, R.c, -o.ro)) * b; });
 }
 
 struct DistillOut {
@@ -1052,6 +1132,8 @@ struct DistillOut {
     long long w_s;
     float scale;
     void* dx;
+    long long keep;  // rows from here on are left in the caches for the backward pass
+    bool nt;         // the gradient is not
 };
 __device__ __forceinline__ float row_weight(const Rows& R, const DistillOut& O, long long r) {
     return (O.w ? O.w[r * O.w_s] : 1.f) * O.scale * R.invT;
@@ -1060,7 +1142,8 @@ __device__ __forceinline__ float row_weight(const Rows& R, const DistillOut& O, 
 // A team a row: statistics, loss and (dx) the gradient.  NV > 0: the row stays in registers (NV vectors a thread)
 // between its two uses, and HBM sees it once; NV = 0: it is read again from the cache.
 template <class T, int TEAM, bool MASK, int NV>
-__global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
+__global__ __launch_bounds__(block_of<TEAM>) __attribute__((amdgpu_waves_per_eu(4)))  // four rows of 64 KB a CU
+void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     extern __shared__ unsigned bits_all[];
     constexpr int TEAMS = block_of<TEAM> / TEAM, N = VN<T>;
     __shared__ Shared sh;
@@ -1072,26 +1155,40 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Te
     const T* x = row_ptr<T>(R, r);
     const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
     const int tid = team_tid<TEAM>(), V = R.V, nvec = V / N, mine = team_in_block<TEAM>();
-    const int words = bit_words<T, TEAM>(V);
+    const int words = bit_words<T, TEAM, NV>(V);
     unsigned* bits = bits_all + mine * words;
     Entries& E = Es[mine];
-    constexpr int U = NV >= GROUP ? GROUP : NV > 0 ? NV : 1, Q = NV > 0 ? NV / U : 1;
+    // the entries' loads first: they are few, and the row's come behind them
+    EntryRegs er;
+    if (tid < 64) er = fetch_entries<T>(Te, r, V, x, mk);
+    constexpr int U = NV * N >= 16 ? 16 / N : 1, Q = NV > 0 ? NV / U : 1;  // 16 logits unpacked at a time
     Loaded<T, U> L[Q];
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) load_group<T, TEAM, U>(L[q], x, tid + q * U * TEAM, nvec);
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {  // past the end: the last vector again, made -inf when it is used
+                const int vi = tid + (q * U + u) * TEAM;
+                L[q].v[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (nvec > 0) L[q].v[u] = load16<true>(x + (long long)(vi < nvec ? vi : nvec - 1) * N);
+            }
     }
-    if (Te.rest)
+    const bool marked = Te.rest || O.dx || O.stats;  // only the loss without rest needs no bits
+    if (marked)
         for (int i = tid; i < words; i += TEAM) bits[i] = 0;
     EntryHead h;
     if (tid < 64) {
-        h = load_entries<T>(E, Te, r, V, x, mk, R.c);
+        h = load_entries<T>(E, er, Te, R.c);
         if (tid == 0) fars[mine] = h.far && Te.rest;
     }
+    bool repeats = false;
     team_sync<TEAM>();
-    if (Te.rest) {
-        if (tid < 64)
-            for (int j = tid; j < Te.k; j += 64) set_bit(bits, E.id[j], 0, V);
+    if (marked) {
+        if (tid < 64) {
+            for (int j = tid; j < Te.k; j += 64) repeats |= set_bit(bits, E.id[j], 0, V);
+            repeats = __ballot(repeats) != 0;
+            if (repeats) find_repeats(E, Te.k);
+        }
         team_sync<TEAM>();
     }
     const SkipBits<T> skip{bits, Te.rest != 0};
@@ -1101,14 +1198,16 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Te
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             float f[U * N], gm = -INFINITY;
+            opaque(L[q]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int vi = tid + (q * U + u) * TEAM;
-                unpack<T>(L[q].v[u], f + u * N);
-                if (vi < nvec) {
-                    if constexpr (MASK) apply_mask<T>(mk + (long long)vi * N, f + u * N);
-                    skip(vi, f + u * N);
-                }
+                const uint4 w = L[q].v[u];
+                constexpr unsigned none = MINF_BITS<T>;
+                unpack<T>(vi < nvec ? w : make_uint4(none, none, none, none), f + u * N);
+                if constexpr (MASK)
+                    if (vi < nvec) apply_mask<T>(mk + vi * N, f + u * N);
+                skip(vi, f + u * N);
 #pragma unroll
                 for (int i = 0; i < N; ++i) gm = nmax(gm, f[u * N + i]);
             }
@@ -1116,8 +1215,8 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Te
             sum_group<false, U * N>(a, f, gm, R.c);
             __builtin_amdgcn_sched_barrier(0);  // one group unpacked at a time
         }
-        const int i = nvec * N + tid;
         if (nvec * N < V) {
+            const int i = nvec * N + tid;
             float f[2] = {-INFINITY, -INFINITY};
             if (i < V && (!MASK || mk[i]) && !skip.one(i)) f[0] = (float)x[i];
             mx = nmax(mx, f[0]);
@@ -1125,58 +1224,67 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_rows_kernel(Rows R, Te
         }
     } else {
         Best none{-INFINITY, 0};
-        row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip);
+        row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
     const Stat v = row_stat<T, TEAM>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
     if (tid < 64) {
-        const Row o = finish_row(R, Te, E, h, v, O.row_loss + r);
+        const Row o = row_coefficients(R, Te, E, h, v, repeats);
         if (tid == 0) {
             rows[mine] = o;
             if (O.stats) ((Row*)O.stats)[r] = o;
         }
     }
-    if (!O.dx) return;
     team_sync<TEAM>();
-    if constexpr (NV > 0 && sizeof(T) == 2) {
-        // hides from the compiler that the packed logits are those already unpacked: it would keep the unpacked
-        // ones, twice the registers, over the reduction
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                asm volatile("" : "+v"(L[q].v[u].x), "+v"(L[q].v[u].y), "+v"(L[q].v[u].z), "+v"(L[q].v[u].w));
+    auto loss = [&] {
+        if (tid < 64) {
+            const float kl = row_kl(R, Te, E, h, rows[mine]);
+            if (tid == 0) O.row_loss[r] = kl;
+        }
+    };
+    if (!O.dx) {
+        loss();
+        return;
     }
+    if constexpr (NV > 0)
+        for (int q = 0; q < Q; ++q) opaque(L[q]);
     const Row o = rows[mine];
     const float g = row_weight(R, O, r);
     T* d = (T*)O.dx + r * (long long)V;
     if (NV > 0 && o.wide == 0.f && o.so != 0.f) {
         const float b = o.b * g / o.so;
+        auto write = [&](auto nt) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q)
+            for (int q = 0; q < Q; ++q)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int vi = tid + (q * U + u) * TEAM;
-                if (vi >= nvec) continue;
-                float y[N];
-                unpack<T>(L[q].v[u], y);
-                if constexpr (MASK) apply_mask<T>(mk + (long long)vi * N, y);
+                for (int u = 0; u < U; ++u) {
+                    const int vi = tid + (q * U + u) * TEAM;
+                    if (vi >= nvec) continue;
+                    float y[N];
+                    unpack<T>(L[q].v[u], y);
+                    if constexpr (MASK) apply_mask<T>(mk + vi * N, y);
 #pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = ex2(__builtin_fmaf(y[i], R.c, -o.ro)) * b;
-                store16(d + (long long)vi * N, y);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    for (int i = 0; i < N; ++i) y[i] = ex2(__builtin_fmaf(y[i], R.c, -o.ro)) * b;
+                    store16<decltype(nt)::value>(d + (long long)vi * N, y);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        };
+        if (O.nt)
+            write(std::true_type{});
+        else
+            write(std::false_type{});
         const int i = nvec * N + tid;
         if (i < V) d[i] = (T)(!MASK || mk[i] ? ex2(__builtin_fmaf((float)x[i], R.c, -o.ro)) * b : 0.f);
     } else {
-        write_outside<T, TEAM, MASK>(R, o, g, x, mk, d, V);
+        write_outside<T, TEAM, MASK>(R, o, g, x, mk, d, V, O.nt);
     }
     team_sync<TEAM>();
     write_entries<T, TEAM>(R, Te, E, o, g, mk, d, 0, V);
+    loss();  // last: the other waves do not wait for it
 }
 
 // a part of a row of few rows: its statistics outside the entries
 template <class T, bool MASK>
-__global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, Split P) {
+__global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, DistillOut O, Split P) {
     extern __shared__ unsigned bits[];
     __shared__ Shared sh;
     const long long r = block_row();
@@ -1202,7 +1310,7 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, S
     Sum a{-FAR, 0.f, 0.f};
     float mx = -INFINITY;
     Best none{-INFINITY, 0};
-    row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0});
+    row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0}, r < O.keep);
     a = team_sum<256>(a, sh.sum);
     const bool plain = plain_sum(a);
     const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
@@ -1225,7 +1333,11 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
     Entries& E = Es[team_in_block<TEAM>()];
     EntryHead h;
-    if (tid < 64) h = load_entries<T>(E, Te, r, R.V, x, mk, R.c);
+    bool repeats = false;
+    if (tid < 64) {
+        h = load_entries<T>(E, fetch_entries<T>(Te, r, R.V, x, mk), Te, R.c);
+        if constexpr (JOIN) repeats = find_repeats(E, Te.k);
+    }
     Row o;
     if constexpr (JOIN) {
         if (tid < 64) {
@@ -1256,11 +1368,14 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
             v = Stat{s.m, s.s, 0.f, true};
         }
         if (tid < 64) {
-            const bool first = blockIdx.z == 0;
-            o = finish_row(R, Te, E, h, v, first ? O.row_loss + r : nullptr);
-            if (tid == 0) {
-                row = o;
-                if (O.stats && first) ((Row*)O.stats)[r] = o;
+            o = row_coefficients(R, Te, E, h, v, repeats);
+            if (tid == 0) row = o;
+            if (blockIdx.z == 0) {
+                const float kl = row_kl(R, Te, E, h, o);
+                if (tid == 0) {
+                    O.row_loss[r] = kl;
+                    if (O.stats) ((Row*)O.stats)[r] = o;
+                }
             }
         }
         if (!O.dx) return;
@@ -1271,7 +1386,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     }
     const float g = row_weight(R, O, r);
     T* d = (T*)O.dx + r * (long long)R.V + from;
-    write_outside<T, TEAM, MASK>(R, o, g, x + from, MASK ? mk + from : nullptr, d, V);
+    write_outside<T, TEAM, MASK>(R, o, g, x + from, MASK ? mk + from : nullptr, d, V, O.nt);
     team_sync<TEAM>();
     write_entries<T, TEAM>(R, Te, E, o, g, MASK ? mk + from : nullptr, d, from, V);
 }
@@ -1332,19 +1447,20 @@ bool teacher_of(const azg_teacher* t, Teacher* Te) {
 }
 
 // Which team takes a row.  A wave: rows of up to 4 KB (a block would leave most of its threads idle).  A block:
-// longer ones.  Parts: rows longer than a block's LDS holds the maxima or bits of, and, where there are fewer rows
+// longer ones.  Parts: rows longer than a block holds the maxima or bits (LDS) or the logits (registers) of, and, where there are fewer rows
 // than would fill the chip, rows of more than 8192 elements, in parts of 4096 or more.
 constexpr int WAVE_BYTES = 4096, PART_MIN = 4096;
 template <class T>
-constexpr int BLOCK_MAX = sizeof(T) == 4 ? 65536 : 131072;
-
+int logprobs_most(bool top) { return top ? 1024 * 16 * VN<T> : 1 << 30; }
 template <class T>
-Split parts_of(const Rows& R) {
+int distill_most(bool grad) { return grad ? 1024 * 16 * VN<T> : 1 << 18; }
+
+Split parts_of(const Rows& R, int most) {
     Split P{nullptr, nullptr, 1, R.V};
-    long long n = (R.V + BLOCK_MAX<T> - 1) / BLOCK_MAX<T>;
+    long long n = (R.V - 1) / most + 1;
     if (R.rows < 128 && R.V > 2 * PART_MIN) {
-        long long want = 512 / R.rows, most = R.V / PART_MIN;
-        if (want > most) want = most;
+        long long want = 512 / R.rows;
+        if (want > R.V / PART_MIN) want = R.V / PART_MIN;
         if (want > n) n = want;
     }
     if (n > 1) {
@@ -1367,11 +1483,23 @@ unsigned gmax_bytes(int V) {
     const int ng = (V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP);
     return (unsigned)((ng + 1) * block_of<TEAM> * 4);
 }
-template <class T, int TEAM>
-unsigned bits_bytes(const Teacher& Te, int V) {
-    return Te.rest ? (unsigned)(bit_words<T, TEAM>(V) * 4 * (block_of<TEAM> / TEAM)) : 0;
+template <class T, int TEAM, int NV = 0>
+unsigned bits_bytes(int V) {
+    return (unsigned)(bit_words<T, TEAM, NV>(V) * 4 * (block_of<TEAM> / TEAM));
 }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// What is read again is worth a place in the Infinity Cache (256 MB): of a forward pass whose backward pass follows the
+// last rows, which that takes first, and of a gradient what fits, for the products that read it next.  All else
+// goes past the caches.
+constexpr long long CACHE_BYTES = 256LL << 20;
+template <class T>
+long long keep_from(const Rows& R, bool backward) {
+    const long long fit = CACHE_BYTES / ((long long)R.V * (int)sizeof(T));
+    return !backward ? R.rows : fit < R.rows ? R.rows - fit : 0;
+}
+template <class T>
+bool too_large(const Rows& R) { return R.rows * R.V * (int)sizeof(T) > CACHE_BYTES / 2; }
 
 constexpr int BWD_LEN = 16384;  // elements of a row that a block of a gradient kernel takes
 
@@ -1390,7 +1518,7 @@ void distill_bwd(const Rows& R, const Teacher& Te, const DistillOut& O, hipStrea
 template <class T, int TEAM, bool MASK, int NV>
 void distill_rows(const Rows& R, const Teacher& Te, const DistillOut& O, hipStream_t st) {
     hipLaunchKernelGGL((distill_rows_kernel<T, TEAM, MASK, NV>), team_grid<TEAM>(R.rows), dim3(block_of<TEAM>),
-                       (bits_bytes<T, TEAM>(Te, R.V)), st, R, Te, O);
+                       (bits_bytes<T, TEAM, NV>(R.V)), st, R, Te, O);
 }
 
 template <class T, bool MASK>
@@ -1400,7 +1528,7 @@ void distill_fwd(const Rows& R, const Teacher& Te, const DistillOut& O, Split P,
     if (P.n > 1) {
         P.part = work;
         hipLaunchKernelGGL((distill_part_kernel<T, MASK>), team_grid<256>(R.rows, P.n), dim3(256),
-                           (bits_bytes<T, 256>(Te, P.len)), st, R, Te, P);
+                           (bits_bytes<T, 256>(P.len)), st, R, Te, O, P);
         hipLaunchKernelGGL((distill_bwd_kernel<T, 256, MASK, true>), team_grid<256>(R.rows, O.dx ? P.n : 1), dim3(256),
                            0, st, R, Te, O, P, P.len);
     } else if (!O.dx) {
@@ -1446,15 +1574,15 @@ extern "C" int64_t azg_logprobs_work(const azg_logits* L, int32_t top) {
     Rows R;
     if (!rows_of(L, &R) || top < 0 || top > TOP_MAX) return bad("azg_logprobs_work: bad argument");
     return by_type(L->dtype, [&](auto z) -> int64_t {
-        const Split P = parts_of<decltype(z)>(R);
+        const Split P = parts_of(R, logprobs_most<decltype(z)>(top > 0));
         return P.n > 1 ? up16(R.rows * P.n * 16) + R.rows * P.n * top * 8 : 0;
     });
 }
-extern "C" int64_t azg_distill_work(const azg_logits* L, int32_t) {
+extern "C" int64_t azg_distill_work(const azg_logits* L, int32_t grad) {
     Rows R;
     if (!rows_of(L, &R)) return bad("azg_distill_work: bad argument");
     return by_type(L->dtype, [&](auto z) -> int64_t {
-        const Split P = parts_of<decltype(z)>(R);
+        const Split P = parts_of(R, distill_most<decltype(z)>(grad));
         return P.n > 1 ? R.rows * P.n * 16 : 0;
     });
 }
@@ -1468,15 +1596,16 @@ extern "C" int azg_logprobs_fwd(const azg_logits* L, const void* actions, int32_
         return bad("azg_logprobs_fwd: bad argument");
     const int64_t need = azg_logprobs_work(L, top);
     if (need > 0 && (!work || work_bytes < need)) return bad("azg_logprobs_fwd: work is too small");
-    const LogprobsOut O{actions, actions64 != 0, top, stats, logp, entropy, lse, top_logp, (long long*)top_ids};
+    LogprobsOut O{actions, actions64 != 0, top, stats, logp, entropy, lse, top_logp, (long long*)top_ids, 0};
     by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
         return by_mask(R, [&](auto m) {
             constexpr bool MASK = decltype(m)::value;
+            O.keep = keep_from<T>(R, stats != nullptr);
             if (top)
-                logprobs_fwd<T, MASK, true>(R, O, parts_of<T>(R), (char*)work, (hipStream_t)stream);
+                logprobs_fwd<T, MASK, true>(R, O, parts_of(R, logprobs_most<T>(true)), (char*)work, (hipStream_t)stream);
             else
-                logprobs_fwd<T, MASK, false>(R, O, parts_of<T>(R), (char*)work, (hipStream_t)stream);
+                logprobs_fwd<T, MASK, false>(R, O, parts_of(R, logprobs_most<T>(false)), (char*)work, (hipStream_t)stream);
             return 0;
         });
     });
@@ -1496,13 +1625,14 @@ extern "C" int azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_
             if (by_wave<T>(R))
                 hipLaunchKernelGGL((logprobs_bwd_kernel<T, 64, MASK>), team_grid<64>(R.rows), dim3(256), 0,
                                    (hipStream_t)stream, R, actions, actions64, stats, g_logp, (long long)g_logp_stride,
-                                   g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx, R.V);
+                                   g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx, R.V,
+                                   too_large<T>(R));
             else
                 hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, MASK>),
                                    team_grid<256>(R.rows, (R.V + BWD_LEN - 1) / BWD_LEN), dim3(256), 0,
                                    (hipStream_t)stream, R, actions, actions64, stats, g_logp, (long long)g_logp_stride,
                                    g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx,
-                                   BWD_LEN);
+                                   BWD_LEN, too_large<T>(R));
             return 0;
         });
     });
@@ -1518,11 +1648,13 @@ extern "C" int azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float*
     const int64_t need = azg_distill_work(L, dx != nullptr);
     if (need > 0 && (!work || work_bytes < need)) return bad("azg_distill_fwd: work is too small");
     hipStream_t st = (hipStream_t)stream;
-    const DistillOut O{stats, row_loss, weight, (long long)weight_stride, scale, dx};
+    DistillOut O{stats, row_loss, weight, (long long)weight_stride, scale, dx, 0, false};
     by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
+        O.keep = keep_from<T>(R, stats != nullptr || dx != nullptr);
+        O.nt = too_large<T>(R);
         return by_mask(R, [&](auto m) {
-            distill_fwd<T, decltype(m)::value>(R, Te, O, parts_of<T>(R), (float4*)work, st);
+            distill_fwd<T, decltype(m)::value>(R, Te, O, parts_of(R, distill_most<T>(dx != nullptr)), (float4*)work, st);
             return 0;
         });
     });
@@ -1537,9 +1669,10 @@ extern "C" int azg_distill_bwd(const azg_logits* L, const azg_teacher* t, const 
     Rows R;
     Teacher Te;
     if (!rows_of(L, &R) || !teacher_of(t, &Te) || !stats || !dx) return bad("azg_distill_bwd: bad argument");
-    const DistillOut O{const_cast<float*>(stats), nullptr, weight, (long long)weight_stride, scale, dx};
+    DistillOut O{const_cast<float*>(stats), nullptr, weight, (long long)weight_stride, scale, dx, 0, false};
     by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
+        O.nt = too_large<T>(R);
         return by_mask(R, [&](auto m) {
             distill_bwd<T, decltype(m)::value>(R, Te, O, (hipStream_t)stream);
             return 0;
