@@ -49,23 +49,6 @@ class Config(ctypes.Structure):
 
 assert ctypes.sizeof(Config) == 64
 
-
-class Logits(ctypes.Structure):
-    """azg_logits: rows of policy logits and their mask (include/azg.h)."""
-    _fields_ = [("x", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("rows", ctypes.c_int64),
-                ("inner", ctypes.c_int64), ("stride_outer", ctypes.c_int64), ("stride_inner", ctypes.c_int64),
-                ("mask_outer", ctypes.c_int64), ("mask_inner", ctypes.c_int64), ("vocab", ctypes.c_int64),
-                ("dtype", ctypes.c_int32), ("temperature", ctypes.c_float)]
-
-
-class Teacher(ctypes.Structure):
-    """azg_teacher: a teacher's k entries per row (include/azg.h)."""
-    _fields_ = [("logp", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("dtype", ctypes.c_int32),
-                ("ids64", ctypes.c_int32), ("k", ctypes.c_int32), ("rest", ctypes.c_int32)]
-
-
-assert ctypes.sizeof(Logits) == 80 and ctypes.sizeof(Teacher) == 32
-
 # (name, restype, argtypes) of every symbol include/azg.h declares
 _VP, _I32, _I64, _U32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32
 SIGNATURES = [
@@ -151,15 +134,15 @@ SIGNATURES = [
     ("azg_train_loss_fwd", ctypes.c_int, [_VP, _I32, _VP, _I32, _VP, _I32, _VP, _I32, _I32, _VP, _VP, _VP]),
     ("azg_train_loss_bwd", ctypes.c_int, [_VP, _I32, _VP, _I32, _VP, _I32, _VP, _VP, _I32, _I32, _VP, _VP, _I32, _VP,
                                           _I32, _VP]),
-    ("azg_logprobs_work", _I64, [ctypes.POINTER(Logits), _I32]),
-    ("azg_distill_work", _I64, [ctypes.POINTER(Logits), _I32]),
-    ("azg_logprobs_fwd", ctypes.c_int, [ctypes.POINTER(Logits), _VP, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+    ("azg_logprobs_work", _I64, [_VP, _I32]),
+    ("azg_distill_work", _I64, [_VP, _I32]),
+    ("azg_logprobs_fwd", ctypes.c_int, [_VP, _VP, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
                                         _I64, _VP]),
-    ("azg_logprobs_bwd", ctypes.c_int, [ctypes.POINTER(Logits), _VP, _I32, _VP, _VP, _I64, _VP, _I64, _VP, _I64, _VP,
+    ("azg_logprobs_bwd", ctypes.c_int, [_VP, _VP, _I32, _VP, _VP, _I64, _VP, _I64, _VP, _I64, _VP,
                                         _VP]),
-    ("azg_distill_fwd", ctypes.c_int, [ctypes.POINTER(Logits), ctypes.POINTER(Teacher), _VP, _VP, _VP, _I64,
+    ("azg_distill_fwd", ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _I64,
                                        ctypes.c_float, _VP, _VP, _VP, _I64, _VP]),
-    ("azg_distill_bwd", ctypes.c_int, [ctypes.POINTER(Logits), ctypes.POINTER(Teacher), _VP, _VP, _I64,
+    ("azg_distill_bwd", ctypes.c_int, [_VP, _VP, _VP, _VP, _I64,
                                        ctypes.c_float, _VP, _VP]),
 ]
 

@@ -17,8 +17,9 @@ number (infinities and NaN there do not matter), its probability and its gradien
 logit of -inf is probability 0; a legal NaN or +inf makes its row's numbers NaN.  All work is queued on
 the current stream of the logits' device; nothing synchronises, and results do not depend on the
 order in which blocks run."""
-import ctypes
+import functools
 import math
+import struct
 from collections import namedtuple
 
 import torch
@@ -32,27 +33,24 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # enum azg_dt
 ActionLogprobs = namedtuple("ActionLogprobs", "logp entropy lse top_logp top_ids")
 
 
+# azg_logits and azg_teacher as bytes (the calls copy them): a fifth of what a ctypes.Structure costs to fill
+_LOGITS = struct.Struct("PPqqqqqqqif").pack
+_TEACHER = struct.Struct("PPiiii").pack
+_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(i).cuda_stream without the Stream object
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """The device guard of a call: its kernels go to the logits' device, whichever is current."""
-    __slots__ = ("dev", "guard")
-
-    def __init__(self, dev):
-        self.dev = dev
-        self.guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.dev.index:
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(device, fn, *args):
+    """fn(*args, stream) on the device of the logits, whichever is current."""
+    i = device.index
+    if torch.cuda.current_device() == i:
+        _lib.check(fn(*args, _stream(i)))
+    else:
+        with torch.cuda.device(i):
+            _lib.check(fn(*args, _stream(i)))
 
 
 def _fold(shape, *strides):
@@ -92,9 +90,7 @@ def _check_logits(name, logits, temperature):
 def _check_mask(name, logits, mask):
     if mask is None:
         return None
-    if mask.dtype is torch.bool:
-        mask = mask.view(torch.uint8)
-    elif mask.dtype is not torch.uint8:
+    if mask.dtype is not torch.bool and mask.dtype is not torch.uint8:
         raise ValueError(f"{name}: mask must be bool or uint8, got {mask.dtype}")
     if mask.device != logits.device:
         raise ValueError(f"{name}: mask on {mask.device}, logits on {logits.device}")
@@ -108,8 +104,12 @@ def _check_mask(name, logits, mask):
 
 
 def _rows(logits, mask, temperature):
-    """(logits, mask, azg_logits): copies only where the strides do not fold."""
+    """(logits, mask, rows, azg_logits): copies only where the strides do not fold."""
     V = logits.shape[-1]
+    n = logits.numel() // V
+    if logits.is_contiguous() and (mask is None or mask.is_contiguous()):
+        return logits, mask, n, _LOGITS(logits.data_ptr(), 0 if mask is None else mask.data_ptr(), n, max(n, 1), 0, V, 0,
+                                        V, V, _DTYPES[logits.dtype], temperature)
     lead = logits.shape[:-1]
     if logits.stride(-1) != 1 and V > 1:
         logits = logits.contiguous()
@@ -126,9 +126,8 @@ def _rows(logits, mask, temperature):
             f = _fold(lead, logits.stride()[:-1], mask.stride()[:-1])
     inner, st = f
     m = st[1] if mask is not None else (0, 0)
-    L = _lib.Logits(logits.data_ptr(), _ptr(mask), logits.numel() // V, inner, st[0][0], st[0][1], m[0], m[1], V,
-                    _DTYPES[logits.dtype], temperature)
-    return logits, mask, L
+    return logits, mask, n, _LOGITS(logits.data_ptr(), _ptr(mask) or 0, n, inner, st[0][0], st[0][1], m[0], m[1], V,
+                                    _DTYPES[logits.dtype], temperature)
 
 
 def _check_ints(name, what, t, shape, device):
@@ -136,7 +135,7 @@ def _check_ints(name, what, t, shape, device):
         raise ValueError(f"{name}: {what} must be int64 or int32, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name}: {what} on {t.device}, logits on {device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: {what} {tuple(t.shape)}, expected {tuple(shape)}")
     return t.contiguous()
 
@@ -152,30 +151,39 @@ def _spread(g):
     return g.contiguous(), 1
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprobs_work(n, V, dtype, top):
+    return _lib.lib().azg_logprobs_work(_LOGITS(1, 0, n, n, 0, 0, 0, 0, V, dtype, 1.0), top)
+
+
+@functools.lru_cache(maxsize=1024)
+def _distill_work(n, V, dtype, grad):
+    return _lib.lib().azg_distill_work(_LOGITS(1, 0, n, n, 0, 0, 0, 0, V, dtype, 1.0), grad)
+
+
 def _work(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _logprobs(logits, actions, top, t, mask, want_stats):
     lead, dev = logits.shape[:-1], logits.device
-    logits, mask, L = _rows(logits, mask, t)
-    n = L.rows
-    out = torch.empty((3 if actions is not None else 2, *lead), dtype=torch.float32, device=dev)
-    entropy, lse = out[0], out[1]
-    logp = out[2] if actions is not None else None
-    top_logp = top_ids = None
+    logits, mask, n, L = _rows(logits, mask, t)
+    logp = top_logp = top_ids = stats = None
+    if actions is None:
+        entropy, lse = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind(0)
+    else:
+        entropy, lse, logp = torch.empty((3, *lead), dtype=torch.float32, device=dev).unbind(0)
     if top:
         top_logp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
         top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-    stats = torch.empty((n, 4), dtype=torch.float32, device=dev) if want_stats else None
+    if want_stats:
+        stats = torch.empty((n, 4), dtype=torch.float32, device=dev)
     if n:
-        lib = _lib.lib()
-        nb = lib.azg_logprobs_work(L, top)
+        nb = _logprobs_work(n, logits.shape[-1], _DTYPES[logits.dtype], top)
         work = _work(nb, dev)
-        with _On(dev) as stream:
-            _lib.check(lib.azg_logprobs_fwd(L, _ptr(actions), actions is not None and actions.dtype is torch.int64, top,
-                                            _ptr(stats), _ptr(logp), entropy.data_ptr(), lse.data_ptr(),
-                                            _ptr(top_logp), _ptr(top_ids), _ptr(work), nb, stream))
+        _call(dev, _lib.lib().azg_logprobs_fwd, L, _ptr(actions), actions is not None and
+              actions.dtype is torch.int64, top, _ptr(stats), _ptr(logp), entropy.data_ptr(), lse.data_ptr(),
+              _ptr(top_logp), _ptr(top_ids), _ptr(work), nb)
     return logits, mask, (logp, entropy, lse, top_logp, top_ids), stats
 
 
@@ -195,14 +203,12 @@ class _ActionLogprobs(torch.autograd.Function):
         logits, mask, actions, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:
             return None, None, None, None, None
-        _, _, L = _rows(logits, mask, ctx.t)
+        _, _, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if dx.numel():
+        if n:
             (a, sa), (e, se), (z, sz) = _spread(g_logp), _spread(g_entropy), _spread(g_lse)
-            with _On(logits.device) as stream:
-                _lib.check(_lib.lib().azg_logprobs_bwd(L, _ptr(actions), actions is not None and
-                                                       actions.dtype is torch.int64, stats.data_ptr(), _ptr(a), sa,
-                                                       _ptr(e), se, _ptr(z), sz, dx.data_ptr(), stream))
+            _call(logits.device, _lib.lib().azg_logprobs_bwd, L, _ptr(actions), actions is not None and
+                  actions.dtype is torch.int64, stats.data_ptr(), _ptr(a), sa, _ptr(e), se, _ptr(z), sz, dx.data_ptr())
         return dx, None, None, None, None
 
 
@@ -228,44 +234,42 @@ def action_logprobs(logits, actions=None, *, top=0, temperature=1.0, mask=None):
     return ActionLogprobs(*_logprobs(logits, actions, top, t, mask, False)[2])
 
 
-def _check_teacher(name, logits, teacher_logp, teacher_ids, rest):
-    lead = tuple(logits.shape[:-1])
+def _check_teacher(name, logits, teacher_logp, teacher_ids):
+    lead = logits.shape[:-1]
     if teacher_logp.dtype not in _DTYPES:
         raise ValueError(f"{name}: teacher_logp must be float32, bfloat16 or float16, got {teacher_logp.dtype}")
-    if teacher_logp.dim() != len(lead) + 1 or tuple(teacher_logp.shape[:-1]) != lead or \
+    if teacher_logp.dim() != len(lead) + 1 or teacher_logp.shape[:-1] != lead or \
             not 1 <= teacher_logp.shape[-1] <= TOP_MAX:
-        raise ValueError(f"{name}: teacher_logp {tuple(teacher_logp.shape)}, expected {lead} + (1 to {TOP_MAX},)")
+        raise ValueError(f"{name}: teacher_logp {tuple(teacher_logp.shape)}, expected {tuple(lead)} + (1 to {TOP_MAX},)")
     if teacher_logp.device != logits.device:
         raise ValueError(f"{name}: teacher_logp on {teacher_logp.device}, logits on {logits.device}")
     if teacher_logp.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: the teacher gets no gradient: detach teacher_logp")
     ids = _check_ints(name, "teacher_ids", teacher_ids, teacher_logp.shape, logits.device)
-    return teacher_logp.detach().contiguous(), ids
+    if teacher_logp.requires_grad:
+        teacher_logp = teacher_logp.detach()
+    return teacher_logp.contiguous(), ids
 
 
 def _teacher(logp, ids, rest):
-    return _lib.Teacher(logp.data_ptr(), ids.data_ptr(), _DTYPES[logp.dtype], ids.dtype is torch.int64,
-                        logp.shape[-1], bool(rest))
+    return _TEACHER(logp.data_ptr(), ids.data_ptr(), _DTYPES[logp.dtype], ids.dtype is torch.int64, logp.shape[-1],
+                    bool(rest))
 
 
 def _distill(logits, mask, t, t_logp, t_ids, rest, weight, scale, want_stats, want_total, want_grad):
     """(row losses, total, gradient, stats) of scale sum_r weight_r KL_r."""
-    lead, dev = logits.shape[:-1], logits.device
-    shape = logits.shape
-    logits, mask, L = _rows(logits, mask, t)
-    n = L.rows
+    lead, dev, shape = logits.shape[:-1], logits.device, logits.shape
+    logits, mask, n, L = _rows(logits, mask, t)
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     total = torch.empty((), dtype=torch.float32, device=dev) if want_total else None
     dx = torch.empty(shape, dtype=logits.dtype, device=dev) if want_grad else None
     stats = torch.empty((n, 8), dtype=torch.float32, device=dev) if want_stats else None
     if n:
         w, ws = _spread(weight)
-        lib = _lib.lib()
-        nb = lib.azg_distill_work(L, want_grad)
+        nb = _distill_work(n, shape[-1], _DTYPES[logits.dtype], want_grad)
         work = _work(nb, dev)
-        with _On(dev) as stream:
-            _lib.check(lib.azg_distill_fwd(L, _teacher(t_logp, t_ids, rest), _ptr(stats), loss.data_ptr(), _ptr(w), ws,
-                                           scale, _ptr(total), _ptr(dx), _ptr(work), nb, stream))
+        _call(dev, _lib.lib().azg_distill_fwd, L, _teacher(t_logp, t_ids, rest), _ptr(stats), loss.data_ptr(), _ptr(w),
+              ws, scale, _ptr(total), _ptr(dx), _ptr(work), nb)
     elif want_total:
         total.zero_()
     return logits, mask, loss, total, dx, stats
@@ -286,13 +290,12 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, mask, t_logp, t_ids, stats = ctx.saved_tensors
-        _, _, L = _rows(logits, mask, ctx.t)
+        _, _, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if dx.numel():
+        if n:
             w, ws = _spread(g)
-            with _On(logits.device) as stream:
-                _lib.check(_lib.lib().azg_distill_bwd(L, _teacher(t_logp, t_ids, ctx.rest), stats.data_ptr(),
-                                                      w.data_ptr(), ws, ctx.scale, dx.data_ptr(), stream))
+            _call(logits.device, _lib.lib().azg_distill_bwd, L, _teacher(t_logp, t_ids, ctx.rest), stats.data_ptr(),
+                  w.data_ptr(), ws, ctx.scale, dx.data_ptr())
         return dx, None, None, None, None, None, None
 
 
@@ -314,7 +317,7 @@ def distill_loss(logits, teacher_logp, teacher_ids, *, temperature=1.0, mask=Non
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"distill_loss: reduction {reduction!r} ('mean', 'sum' or 'none')")
     mask = _check_mask("distill_loss", logits, mask)
-    t_logp, t_ids = _check_teacher("distill_loss", logits, teacher_logp, teacher_ids, rest)
+    t_logp, t_ids = _check_teacher("distill_loss", logits, teacher_logp, teacher_ids)
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillLoss.apply(logits, t_logp, t_ids, t, mask, bool(rest), reduction)
     n = logits.numel() // logits.shape[-1]
@@ -331,24 +334,24 @@ def distill_loss_grad(logits, teacher_logp, teacher_ids, *, temperature=1.0, mas
     logits.backward(gradient).  No autograd graph is built."""
     t = _check_logits("distill_loss_grad", logits, temperature)
     mask = _check_mask("distill_loss_grad", logits, mask)
-    with torch.no_grad():
-        t_logp, t_ids = _check_teacher("distill_loss_grad", logits, teacher_logp, teacher_ids, rest)
-        n = logits.numel() // logits.shape[-1]
-        w, scale = None, 1.0
-        if weight is None:
-            scale = 1.0 / max(n, 1)
-        elif isinstance(weight, torch.Tensor):
-            if weight.device != logits.device or not weight.is_floating_point():
-                raise ValueError("distill_loss_grad: weight must be a floating-point tensor on the logits' device")
-            if weight.dim() and weight.shape != logits.shape[:-1]:
-                raise ValueError(f"distill_loss_grad: weight {tuple(weight.shape)}, expected "
-                                 f"{tuple(logits.shape[:-1])} or one number")
-            w = weight.detach()
-        else:
-            scale = float(weight)
-            if not math.isfinite(scale):
-                raise ValueError(f"distill_loss_grad: weight {weight}")
-        _, _, _, total, dx, _ = _distill(logits.detach(), mask, t, t_logp, t_ids, rest, w, scale, False, True, True)
+    t_logp, t_ids = _check_teacher("distill_loss_grad", logits, teacher_logp, teacher_ids)
+    w, scale = None, 1.0
+    if weight is None:
+        scale = 1.0 / max(logits.numel() // logits.shape[-1], 1)
+    elif isinstance(weight, torch.Tensor):
+        if weight.device != logits.device or not weight.is_floating_point():
+            raise ValueError("distill_loss_grad: weight must be a floating-point tensor on the logits' device")
+        if weight.dim() and weight.shape != logits.shape[:-1]:
+            raise ValueError(f"distill_loss_grad: weight {tuple(weight.shape)}, expected "
+                             f"{tuple(logits.shape[:-1])} or one number")
+        w = weight.detach()
+    else:
+        scale = float(weight)
+        if not math.isfinite(scale):
+            raise ValueError(f"distill_loss_grad: weight {weight}")
+    if logits.requires_grad:
+        logits = logits.detach()
+    _, _, _, total, dx, _ = _distill(logits, mask, t, t_logp, t_ids, rest, w, scale, False, True, True)
     return total, dx
 
 

@@ -1,6 +1,7 @@
 """azg_amd.policy without a GPU: its refusals, how leading dimensions fold into rows, and the C entries' checks."""
 import ctypes
 import math
+import struct
 
 import pytest
 import torch
@@ -34,11 +35,11 @@ def test_argument_checks():
     with pytest.raises(ValueError, match="expected"):
         policy._check_ints("f", "actions", torch.zeros(4, dtype=torch.int64), (3,), x.device)
     t, i = torch.zeros((3, 2)), torch.zeros((3, 2), dtype=torch.int64)
-    policy._check_teacher("f", x, t, i, False)
+    policy._check_teacher("f", x, t, i)
     for bt, bi in ((t[:2], i[:2]), (t, i[:, :1]), (t.double(), i), (t, i.float()), (t[:, :0], i[:, :0]),
                    (t.repeat(1, 65), i.repeat(1, 65)), (t.clone().requires_grad_(True), i)):
         with pytest.raises(ValueError):
-            policy._check_teacher("f", x, bt, bi, False)
+            policy._check_teacher("f", x, bt, bi)
 
 
 @pytest.mark.parametrize("make", [
@@ -58,14 +59,16 @@ def test_rows_reach_every_element(make, masked):
         mask = torch.ones(5, dtype=torch.uint8).expand(x.shape)
     elif masked == 2:
         mask = (torch.rand(x.shape) < 0.5).to(torch.uint8)
-    y, m, L = policy._rows(x, mask, 1.0)
-    assert L.vocab == 5 and L.rows * 5 == x.numel() and torch.equal(y, x)
-    for t, so, si, size in ((y, L.stride_outer, L.stride_inner, 4), (m, L.mask_outer, L.mask_inner, 1)):
+    y, m, n, L = policy._rows(x, mask, 1.0)
+    _, _, rows, inner, so, si, mo, mi, vocab, dtype, temp = struct.unpack("PPqqqqqqqif", L)
+    assert len(L) == 80 and vocab == 5 and rows == n and n * 5 == x.numel() and torch.equal(y, x)
+    assert (dtype, temp) == (0, 1.0)
+    for t, so, si, size in ((y, so, si, 4), (m, mo, mi, 1)):
         if t is None:
             continue
         base = t.data_ptr()
         for r, row in enumerate(t.reshape(-1, 5) if t.numel() else []):
-            off = (r // L.inner) * so + (r % L.inner) * si
+            off = (r // inner) * so + (r % inner) * si
             got = (ctypes.c_float if size == 4 else ctypes.c_uint8).from_address(base + off * size).value
             assert got == float(row[0])
 
@@ -76,16 +79,16 @@ def test_c_entries_refuse():
     f = torch.zeros(64)
 
     def logits(**kw):
-        d = dict(x=x.data_ptr(), mask=None, rows=2, inner=2, stride_outer=0, stride_inner=5, mask_outer=0, mask_inner=0,
+        d = dict(x=x.data_ptr(), mask=0, rows=2, inner=2, stride_outer=0, stride_inner=5, mask_outer=0, mask_inner=0,
                  vocab=5, dtype=0, temperature=1.0)
         d.update(kw)
-        return _lib.Logits(*d.values())
+        return policy._LOGITS(*d.values())
 
     p = f.data_ptr()
-    bad = [dict(x=None), dict(rows=0), dict(rows=2 ** 40), dict(inner=0), dict(vocab=0), dict(vocab=2 ** 31),
+    bad = [dict(x=0), dict(rows=0), dict(rows=2 ** 40), dict(inner=0), dict(vocab=0), dict(vocab=2 ** 31),
            dict(dtype=3), dict(dtype=-1), dict(temperature=0.0), dict(temperature=math.nan), dict(temperature=math.inf),
            dict(temperature=-1.0)]
-    t = _lib.Teacher(p, p, 0, 1, 3, 0)
+    t = policy._TEACHER(p, p, 0, 1, 3, 0)
     for kw in bad:
         g = logits(**kw)
         assert L.azg_logprobs_fwd(g, None, 0, 0, None, None, p, p, None, None, None, 0, None) == -1, kw
@@ -103,10 +106,10 @@ def test_c_entries_refuse():
         assert L.azg_logprobs_fwd(g, *a, None, 0, None) == -1, a
     assert L.azg_logprobs_bwd(g, None, 0, p, p, 0, None, 0, None, 0, p, None) == -1  # g_logp without actions
     assert L.azg_logprobs_bwd(g, None, 0, None, None, 0, p, 0, None, 0, p, None) == -1
-    for k in (dict(logp=None), dict(ids=None), dict(dtype=3), dict(k=0), dict(k=129)):
+    for k in (dict(logp=0), dict(ids=0), dict(dtype=3), dict(k=0), dict(k=129)):
         d = dict(logp=p, ids=p, dtype=0, ids64=1, k=3, rest=0)
         d.update(k)
-        u = _lib.Teacher(*d.values())
+        u = policy._TEACHER(*d.values())
         assert L.azg_distill_fwd(g, u, p, p, None, 0, 1.0, None, p, None, 0, None) == -1
         assert L.azg_distill_bwd(g, u, p, None, 0, 1.0, p, None) == -1
     # rows in parts need their scratch memory
