@@ -320,7 +320,7 @@ __device__ __forceinline__ unsigned key_index(unsigned long long key) { return 0
 // ln s in f64 for f32 s > 0: s = 2^e f, f in [0.75, 1.5), ln f = 2 atanh(u), u = (f - 1) / (f + 1), |u| <= 0.2,
 // by its power series to u^15 (what is left is under 2e-13)
 __device__ __forceinline__ double ln_f64(float s) {
-    if (!(s > 0.f) || s == INFINITY) return s == 0.f ? -INFINITY : (double)s;
+    if (!(s > 0.f && s < INFINITY)) return s == 0.f ? -INFINITY : s == INFINITY ? INFINITY : NAN;
     int e;
     float f = frexpf(s, &e);
     if (f < 0.75f) {
@@ -348,20 +348,6 @@ template <class T, int U>
 struct Loaded {
     uint4 v[U];
 };
-template <class T, int TEAM, int U, bool NT>
-__device__ __forceinline__ void load_group(Loaded<T, U>& L, const T* x, int vi, int nvec) {
-    if (vi - team_tid<TEAM>() + TEAM * U <= nvec) {  // the whole team's
-#pragma unroll
-        for (int u = 0; u < U; ++u) L.v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * VN<T>);
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            L.v[u] = make_uint4(MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>);
-            if (vi + u * TEAM < nvec) L.v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * VN<T>);
-        }
-    }
-}
-
 // Hides from the compiler what these registers hold: it would unpack all groups at once, and keep the unpacked
 // logits (twice the registers) from one use to the next.
 template <class T, int U>
@@ -384,39 +370,60 @@ struct NoEdit {
 };
 
 template <class T, int TEAM, bool MASK, bool ENT, bool TOP, bool NT, class Edit>
-__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx,
-                                         Best& best, float* gmax, const Edit& edit) {
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx, Best& best,
+                                         float* gmax, const Edit& edit) {
     constexpr int N = VN<T>;
     const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
-    int g = 0;
-    for (int vi = tid; vi - tid < nvec; vi += step, ++g) {
-        Loaded<T, GROUP> L;
-        load_group<T, TEAM, GROUP, NT>(L, x, vi, nvec);
-        float f[GROUP * N], vm[GROUP];
+    // a vector's elements and maximum
+    auto take = [&](const uint4& v, int vi, float* f) {
+        unpack<T>(v, f);
+        if constexpr (MASK)
+            if (vi < nvec) apply_mask<T>(mk + vi * N, f);
+        edit(vi, f);
+        float m = f[0];
 #pragma unroll
-        for (int u = 0; u < GROUP; ++u) {
-            unpack<T>(L.v[u], f + u * N);
-            if constexpr (MASK)
-                if (vi + u * TEAM < nvec) apply_mask<T>(mk + (vi + u * TEAM) * N, f + u * N);
-            edit(vi + u * TEAM, f + u * N);
-            float m = f[u * N];
-#pragma unroll
-            for (int i = 1; i < N; ++i) m = nmax(m, f[u * N + i]);
-            vm[u] = m;
-            if constexpr (TOP) {
-                const bool up = m > best.v;
-                best.v = up ? m : best.v;
-                best.last = up ? (vi + u * TEAM) * N + N - 1 : best.last;
-            }
+        for (int i = 1; i < N; ++i) m = nmax(m, f[i]);
+        if constexpr (TOP) {
+            const bool up = m > best.v;
+            best.v = up ? m : best.v;
+            best.last = up ? vi * N + N - 1 : best.last;
         }
-        float gm = vm[0];
+        return m;
+    };
+    int g = 0, vi = tid;
+    for (; vi - tid + step <= nvec; vi += step, ++g) {
+        uint4 v[GROUP];
 #pragma unroll
-        for (int u = 1; u < GROUP; ++u) gm = nmax(gm, vm[u]);
+        for (int u = 0; u < GROUP; ++u) v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * N);
+        float f[GROUP * N], gm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) gm = nmax(gm, take(v[u], vi + u * TEAM, f + u * N));
         mx = nmax(mx, gm);
         if constexpr (TOP) gmax[g * TEAM + tid] = gm;
         sum_group<ENT, GROUP * N>(a, f, gm, c);
     }
-    float f[2] = {-INFINITY, -INFINITY};
+    const int left = nvec - (vi - tid);  // the last group: only as many vectors as it has
+    if (left > 0) {
+        uint4 v[GROUP];
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) {
+            v[u] = make_uint4(MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>, MINF_BITS<T>);
+            if (vi + u * TEAM < nvec) v[u] = load16<NT>(x + (long long)(vi + u * TEAM) * N);
+        }
+        float gm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u)
+            if (u * TEAM < left) {
+                float f[N];
+                const float m = take(v[u], vi + u * TEAM, f);
+                gm = nmax(gm, m);
+                sum_group<ENT, N>(a, f, m, c);
+            }
+        mx = nmax(mx, gm);
+        if constexpr (TOP) gmax[g * TEAM + tid] = gm;
+        ++g;
+    }
+    float f[2] = {-INFINITY, -INFINITY};  // what is behind the last vector, an element a thread
     const int i = nvec * N + tid;
     if (i < V && (!MASK || mk[i]) && !edit.one(i)) f[0] = (float)x[i];
     if constexpr (TOP) {
@@ -803,27 +810,39 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
 template <class T, int TEAM, bool MASK, bool NT, class F>
 __device__ __forceinline__ void map_row(const T* x, const uint8_t* mk, T* d, int V, F f) {
     constexpr int N = VN<T>;
-    const int tid = team_tid<TEAM>(), nvec = V / N;
-    for (int vi = tid; vi - tid < nvec; vi += TEAM * GROUP) {
-        Loaded<T, GROUP> L;
-        load_group<T, TEAM, GROUP, true>(L, x, vi, nvec);
+    const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
+    auto put = [&](const uint4& v, int vi) {
+        float y[N];
+        unpack<T>(v, y);
+        if constexpr (MASK) {
+            uint8_t b[N];
+            __builtin_memcpy(b, mk + vi * N, N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = b[i] ? f(y[i], vi * N + i) : 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = f(y[i], vi * N + i);
+        }
+        store16<NT>(d + (long long)vi * N, y);
+    };
+    int vi = tid;
+    for (; vi - tid + step <= nvec; vi += step) {
+        uint4 v[GROUP];
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) v[u] = load16<true>(x + (long long)(vi + u * TEAM) * N);
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u) put(v[u], vi + u * TEAM);
+    }
+    if (vi - tid < nvec) {
+        uint4 v[GROUP];
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
-            const int i0 = (vi + u * TEAM) * N;
-            if (vi + u * TEAM >= nvec) continue;
-            float y[N];
-            unpack<T>(L.v[u], y);
-            if constexpr (MASK) {
-                uint8_t b[N];
-                __builtin_memcpy(b, mk + i0, N);
-#pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = b[i] ? f(y[i], i0 + i) : 0.f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = f(y[i], i0 + i);
-            }
-            store16<NT>(d + i0, y);
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (vi + u * TEAM < nvec) v[u] = load16<true>(x + (long long)(vi + u * TEAM) * N);
         }
+#pragma unroll
+        for (int u = 0; u < GROUP; ++u)
+            if (vi + u * TEAM < nvec) put(v[u], vi + u * TEAM);
     }
     const int i = nvec * N + tid;
     if (i < V) d[i] = (T)(!MASK || mk[i] ? f((float)x[i], i) : 0.f);
@@ -912,6 +931,8 @@ __device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long 
         const int j = lane + 64 * u;
         e.t[u] = -INFINITY;
         e.id[u] = -1;
+        e.x[u] = 0.f;
+        e.legal[u] = false;
         if (j < Te.k) {
             const long long o = r * Te.k + j;
             const long long i = Te.ids64 ? ((const long long*)Te.ids)[o] : ((const int*)Te.ids)[o];
@@ -923,6 +944,7 @@ __device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long 
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+        if (64 * u >= Te.k) continue;
         const int i = e.id[u] < 0 ? 0 : e.id[u];
         e.x[u] = (float)x[i];
         e.legal[u] = !mk || mk[i];
@@ -949,6 +971,8 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
     h.qs = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+        q[u] = 0.f;
+        if (64 * u >= Te.k) continue;
         q[u] = id[u] >= 0 ? expf(e.t[u] - h.tm) : 0.f;
         h.qs += q[u];
     }
@@ -958,6 +982,7 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
+        if (64 * u >= Te.k) continue;
         q[u] *= iq;
         h.Q += q[u];
         if (j < Te.k) {
@@ -1013,7 +1038,8 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int j = lane + 64 * u;
-            xj[u] = j < Te.k && E.first[j] ? E.x[j] : -INFINITY;
+            xj[u] = -INFINITY;
+            if (j < Te.k && E.first[j]) xj[u] = E.x[j];
             mx = nmax(mx, xj[u]);
         }
         mx = wave_max(mx);
@@ -1051,12 +1077,15 @@ __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const 
     const int lane = threadIdx.x & 63;
     const bool wide = o.wide != 0.f;
     const double cd = R.c, ln2 = 0.69314718055994530942;
-    const double lns = ln_f64(o.sa), lnq = Te.rest ? 0.0 : ln_f64(h.qs);
+    // the row's logarithms at once, one a lane: of the sums over all and outside, of the entries' sum, of what is left
+    const double qr = 1.0 - h.Q;
+    const double ln = ln_f64(lane == 0 ? o.sa : lane == 1 ? o.so : lane == 2 ? h.qs : (float)qr);
+    const double lns = lane_of(ln, 0), lnq = Te.rest ? 0.0 : lane_of(ln, 2);
     double loss = 0.0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
-        if (j >= Te.k || E.id[j] < 0) continue;
+        if (64 * u >= Te.k || j >= Te.k || E.id[j] < 0) continue;
         const double q = E.q[j];
         const double lq = ((double)E.t[j] - (double)h.tm) - lnq;
         const double uj = wide ? ((double)E.x[j] - (double)o.ra) * cd : (double)E.x[j] * cd - (double)o.ra;
@@ -1064,8 +1093,8 @@ __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const 
     }
     loss = wave_sum(loss);
     if (Te.rest && o.so != 0.f) {
-        const double qr = 1.0 - h.Q, d = wide ? ((double)o.ro - (double)o.ra) * cd : (double)o.ro - (double)o.ra;
-        if (!(qr <= 0.0)) loss += qr * (ln_f64((float)qr) - (d * ln2 + ln_f64(o.so) - lns));
+        const double d = wide ? ((double)o.ro - (double)o.ra) * cd : (double)o.ro - (double)o.ra;
+        if (!(qr <= 0.0)) loss += qr * (lane_of(ln, 3) - (d * ln2 + lane_of(ln, 1) - lns));
     }
     return (float)loss;
 }
@@ -1170,7 +1199,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
             for (int u = 0; u < U; ++u) {  // past the end: the last vector again, made -inf when it is used
                 const int vi = tid + (q * U + u) * TEAM;
                 L[q].v[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (nvec > 0) L[q].v[u] = load16<true>(x + (long long)(vi < nvec ? vi : nvec - 1) * N);
+                if ((q * U + u) * TEAM < nvec) L[q].v[u] = load16<true>(x + (long long)(vi < nvec ? vi : nvec - 1) * N);
             }
     }
     const bool marked = Te.rest || O.dx || O.stats;  // only the loss without rest needs no bits
@@ -1197,6 +1226,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     if constexpr (NV > 0) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
+            if (q * U * TEAM >= nvec) continue;  // the same for the whole team
             float f[U * N], gm = -INFINITY;
             opaque(L[q]);
 #pragma unroll
@@ -1258,7 +1288,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int vi = tid + (q * U + u) * TEAM;
-                    if (vi >= nvec) continue;
+                    if ((q * U + u) * TEAM >= nvec || vi >= nvec) continue;
                     float y[N];
                     unpack<T>(L[q].v[u], y);
                     if constexpr (MASK) apply_mask<T>(mk + vi * N, y);
@@ -1449,7 +1479,7 @@ bool teacher_of(const azg_teacher* t, Teacher* Te) {
 // Which team takes a row.  A wave: rows of up to 4 KB (a block would leave most of its threads idle).  A block:
 // longer ones.  Parts: rows longer than a block holds the maxima or bits (LDS) or the logits (registers) of, and, where there are fewer rows
 // than would fill the chip, rows of more than 8192 elements, in parts of 4096 or more.
-constexpr int WAVE_BYTES = 4096, PART_MIN = 4096;
+constexpr int WAVE_BYTES = 4096, WAVE_ROWS = 2048, PART_MIN = 4096;
 template <class T>
 int logprobs_most(bool top) { return top ? 1024 * 16 * VN<T> : 1 << 30; }
 template <class T>
@@ -1470,7 +1500,9 @@ Split parts_of(const Rows& R, int most) {
     return P;
 }
 template <class T>
-bool by_wave(const Rows& R) { return (long long)R.V * (int)sizeof(T) <= WAVE_BYTES; }
+bool by_wave(const Rows& R) {
+    return (long long)R.V * (int)sizeof(T) <= (R.rows >= WAVE_ROWS ? 4 * WAVE_BYTES : WAVE_BYTES);
+}
 
 template <int TEAM>
 dim3 team_grid(long long rows, int z = 1) {
