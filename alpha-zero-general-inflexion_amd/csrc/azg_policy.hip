@@ -500,6 +500,35 @@ struct TopShare {
     unsigned long long bound;
 };
 
+// The k-th largest of a wave's words, or less where that needs fewer steps (in any case k words are at least as
+// large): a binary digit a step, counted by ballot.  *wanted: how many of the words equal to it are among the k,
+// 0 if all are.
+__device__ __forceinline__ unsigned kth_word(unsigned w, int k, int* wanted) {
+    unsigned t = 0;
+    int above = 0;
+    *wanted = 0;
+    for (int d = 31; d >= 0; --d) {
+        const unsigned u = t | (1u << d);
+        const int n = __popcll(__ballot(w >= u));
+        if (n == k) return u;
+        if (n > k)
+            t = u;
+        else
+            above = n;
+    }
+    *wanted = k - above;
+    return t;
+}
+__device__ __forceinline__ unsigned long long kth_pair(unsigned long long key, int k) {
+    const unsigned w = (unsigned)(key >> 32);
+    if (__popcll(__ballot(w != 0)) < k) return 0;
+    int wanted;
+    const unsigned t = kth_word(w, k, &wanted);
+    if (wanted == 0) return (unsigned long long)t << 32;
+    const unsigned low = kth_word(w == t ? (unsigned)key : 0u, wanted, &wanted);  // equal values: by index
+    return ((unsigned long long)t << 32) | low;
+}
+
 template <int G>
 __device__ __forceinline__ int rank_in(const unsigned long long* arr, unsigned long long me) {
     int rank = 0;
@@ -508,34 +537,36 @@ __device__ __forceinline__ int rank_in(const unsigned long long* arr, unsigned l
     return rank;
 }
 
+// a bound of the k-th largest of a row from its threads' best.  A wave by ballots (75 us against 82 with ranks, 65536 x
+// 343 f32, top 16: the fewest instructions).  A block by ranks in LDS, each wave for itself over 64 groups of
+// threads where these are enough (the shorter chain: 91 us against 98, 8192 x 32768 bf16, top 8), else over all.
 template <int TEAM>
 __device__ __forceinline__ unsigned long long kth_best(unsigned long long best, int k, TopShare<TEAM>& S) {
     const int tid = team_tid<TEAM>(), lane = threadIdx.x & 63;
-    unsigned long long* arr = S.cand;
     if (tid == 0) S.nh = 0, S.nc = 0, S.bound = 0;
-    if (TEAM == 64 || k <= 32) {  // 64 groups of TEAM / 64 threads, every wave for itself
-        if (k > 64) {
-            team_sync<TEAM>();
-            return 0;
+    if constexpr (TEAM == 64) {
+        team_sync<64>();
+        return k > 64 ? 0 : kth_pair(best, k);
+    } else {
+        static_assert(TEAM == 256, "groups of a quad");
+        unsigned long long* arr = S.cand;
+        if (k <= 32) {
+            auto mx = [](unsigned long long a, unsigned long long b) { return a > b ? a : b; };
+            best = mx(best, dpp<QUAD_XOR1>(best));
+            best = mx(best, dpp<QUAD_XOR2>(best));
+            if ((tid & 3) == 0) arr[tid / 4] = best;
+            __syncthreads();
+            const unsigned long long me = arr[lane];
+            const unsigned long long at = __ballot(me != 0 && rank_in<64>(arr, me) == k - 1);
+            __syncthreads();  // arr becomes the candidates
+            return at ? lane_of(me, __builtin_ctzll(at)) : 0;
         }
-        auto mx = [](unsigned long long a, unsigned long long b) { return a > b ? a : b; };
-        constexpr int P = TEAM / 64;
-        if constexpr (P >= 2) best = mx(best, dpp<QUAD_XOR1>(best));
-        if constexpr (P >= 4) best = mx(best, dpp<QUAD_XOR2>(best));
-        static_assert(P <= 4, "groups of at most a quad");
-        if (P == 1 || (tid & (P - 1)) == 0) arr[tid / P] = best;
-        team_sync<TEAM>();
-        const unsigned long long me = arr[lane];
-        const int rank = rank_in<64>(arr, me);
-        const unsigned long long at = __ballot(me != 0 && rank == k - 1);
-        if (TEAM > 64) __syncthreads();  // arr becomes the candidates
-        return at ? lane_of(me, __builtin_ctzll(at)) : 0;
+        arr[tid] = best;
+        __syncthreads();
+        if (best != 0 && rank_in<TEAM>(arr, best) == k - 1) S.bound = best;
+        __syncthreads();
+        return S.bound;
     }
-    arr[tid] = best;
-    team_sync<TEAM>();
-    if (best != 0 && rank_in<TEAM>(arr, best) == k - 1) S.bound = best;
-    team_sync<TEAM>();
-    return S.bound;
 }
 
 template <class T, int TEAM>
@@ -603,8 +634,9 @@ __device__ int top_select(const T* x, const uint8_t* mk, int V, int k, bool plai
         team_sync<TEAM>();
         const int nh = S.nh;
         if (nh <= S.HITS) {
-            for (int i = tid; i < nh * GROUP; i += TEAM) {
-                const int h = S.hits[i / GROUP], u = i % GROUP, g = h / TEAM, t = h % TEAM;
+            const int per = nvec >= TEAM * GROUP ? GROUP : nvec > TEAM ? (nvec + TEAM - 1) / TEAM : 1;  // vectors a group has
+            for (int i = tid; i < nh * per; i += TEAM) {
+                const int h = S.hits[i / per], u = i % per, g = h / TEAM, t = h % TEAM;
                 float f[N];
                 int i0, n = 0;
                 if (g == ng) {
@@ -995,7 +1027,7 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
             E.first[j] = true;
         }
     }
-    h.Q = wave_sum(h.Q);
+    if (Te.rest) h.Q = wave_sum(h.Q);  // else it is 1
     h.far = __ballot(far) != 0;
     team_sync<64>();
     return h;
@@ -1059,7 +1091,7 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
             all = e;
         }
     }
-    double S = h.Q, qr = 0.0;
+    double S = Te.rest ? h.Q : 1.0, qr = 0.0;
     if (Te.rest && v.s != 0.f) {
         qr = 1.0 - h.Q;
         if (qr < 0.0) qr = 0.0;
@@ -1476,16 +1508,35 @@ bool teacher_of(const azg_teacher* t, Teacher* Te) {
     return true;
 }
 
+// What is read again is worth a place in the Infinity Cache (256 MB): of a forward pass whose backward pass follows the
+// last rows, which that takes first, and of a gradient what fits, for the products that read it next.  All else
+// goes past the caches.
+constexpr long long CACHE_BYTES = 256LL << 20;
+template <class T>
+long long keep_from(const Rows& R, bool backward) {
+    const long long fit = CACHE_BYTES / ((long long)R.V * (int)sizeof(T));
+    return !backward ? R.rows : fit < R.rows ? R.rows - fit : 0;
+}
+template <class T>
+bool too_large(const Rows& R) { return R.rows * R.V * (int)sizeof(T) > CACHE_BYTES / 2; }
+
 // Which team takes a row.  A wave: rows of up to 4 KB (a block would leave most of its threads idle).  A block:
 // longer ones.  Parts: rows longer than a block holds the maxima or bits (LDS) or the logits (registers) of, and, where there are fewer rows
 // than would fill the chip, rows of more than 8192 elements, in parts of 4096 or more.
 constexpr int WAVE_BYTES = 4096, WAVE_ROWS = 2048, PART_MIN = 4096;
 template <class T>
 int logprobs_most(bool top) { return top ? 1024 * 16 * VN<T> : 1 << 30; }
+// With the gradient, rows for which one block would fill a CU's registers alone are taken in parts also where all of
+// the logits fit the Infinity Cache, from which the second kernel reads them (102 us against 116, 1055 x 83523 bf16;
+// beyond it the registers are the better: 255 us, 2048 x 131072 bf16, 1.05 of three passes' time at 5.2 TB/s).
 template <class T>
-int distill_most(bool grad) { return grad ? 1024 * 16 * VN<T> : 1 << 18; }
+long long distill_most(const Rows& R, bool grad) {
+    if (!grad) return 1 << 18;
+    const bool alone = R.V > 512 * 16 * VN<T> && R.rows * R.V * (int)sizeof(T) <= CACHE_BYTES;
+    return (alone ? 512 : 1024) * 16 * VN<T>;
+}
 
-Split parts_of(const Rows& R, int most) {
+Split parts_of(const Rows& R, long long most) {
     Split P{nullptr, nullptr, 1, R.V};
     long long n = (R.V - 1) / most + 1;
     if (R.rows < 128 && R.V > 2 * PART_MIN) {
@@ -1520,18 +1571,6 @@ unsigned bits_bytes(int V) {
     return (unsigned)(bit_words<T, TEAM, NV>(V) * 4 * (block_of<TEAM> / TEAM));
 }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
-
-// What is read again is worth a place in the Infinity Cache (256 MB): of a forward pass whose backward pass follows the
-// last rows, which that takes first, and of a gradient what fits, for the products that read it next.  All else
-// goes past the caches.
-constexpr long long CACHE_BYTES = 256LL << 20;
-template <class T>
-long long keep_from(const Rows& R, bool backward) {
-    const long long fit = CACHE_BYTES / ((long long)R.V * (int)sizeof(T));
-    return !backward ? R.rows : fit < R.rows ? R.rows - fit : 0;
-}
-template <class T>
-bool too_large(const Rows& R) { return R.rows * R.V * (int)sizeof(T) > CACHE_BYTES / 2; }
 
 constexpr int BWD_LEN = 16384;  // elements of a row that a block of a gradient kernel takes
 
@@ -1614,7 +1653,7 @@ extern "C" int64_t azg_distill_work(const azg_logits* L, int32_t grad) {
     Rows R;
     if (!rows_of(L, &R)) return bad("azg_distill_work: bad argument");
     return by_type(L->dtype, [&](auto z) -> int64_t {
-        const Split P = parts_of(R, distill_most<decltype(z)>(grad));
+        const Split P = parts_of(R, distill_most<decltype(z)>(R, grad));
         return P.n > 1 ? R.rows * P.n * 16 : 0;
     });
 }
@@ -1686,7 +1725,7 @@ extern "C" int azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float*
         O.keep = keep_from<T>(R, stats != nullptr || dx != nullptr);
         O.nt = too_large<T>(R);
         return by_mask(R, [&](auto m) {
-            distill_fwd<T, decltype(m)::value>(R, Te, O, parts_of(R, distill_most<T>(dx != nullptr)), (float4*)work, st);
+            distill_fwd<T, decltype(m)::value>(R, Te, O, parts_of(R, distill_most<T>(R, dx != nullptr)), (float4*)work, st);
             return 0;
         });
     });
