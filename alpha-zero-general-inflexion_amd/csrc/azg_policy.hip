@@ -141,7 +141,7 @@ constexpr unsigned MINF_BITS = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, 
 // NT: without a place in the caches, for what is not read again (6.4 TB/s against 5.6, 4096 x 65536 f16)
 template <bool NT, class T>
 __device__ __forceinline__ uint4 load16(const T* p) {
-    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T)), may_alias));
     W w;
     if constexpr (NT)
         w = __builtin_nontemporal_load((const W*)p);
@@ -167,7 +167,7 @@ __device__ __forceinline__ void unpack(const uint4& v, float* f) {
 }
 template <bool NT, class T>
 __device__ __forceinline__ void store16(T* p, const float* f) {
-    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    using W = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T)), may_alias));
     T t[VN<T>];
 #pragma unroll
     for (int i = 0; i < VN<T>; ++i) t[i] = (T)f[i];  // round to nearest even
@@ -223,11 +223,11 @@ __device__ __forceinline__ Sum move_sum(Sum a, float r) {  // to a reference r >
     const int k = (int)fmaxf(d, -4096.f);
     return Sum{r, __builtin_amdgcn_ldexpf(a.s, k), __builtin_amdgcn_ldexpf(__builtin_fmaf(d, a.s, a.w), k)};
 }
-template <int TEAM>
+template <int TEAM, bool ENT>
 __device__ __forceinline__ Sum team_sum(Sum a, Sum* sh) {
     a = move_sum(a, wave_max(a.r));
     a.s = wave_sum(a.s);
-    a.w = wave_sum(a.w);
+    if constexpr (ENT) a.w = wave_sum(a.w);
     if constexpr (TEAM > 64) {
         constexpr int W = TEAM / 64;
         if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
@@ -472,10 +472,10 @@ union Shared {  // one reduction at a time
 };
 
 // a row's statistics from its pass: as they are, or by the element-wise pass; an empty row has s = 0
-template <class T, int TEAM, class Skip>
+template <class T, int TEAM, bool ENT, class Skip>
 __device__ __forceinline__ Stat row_stat(Sum a, float mx, const T* x, const uint8_t* mk, int V, float c, Shared& sh,
                                          bool again, Skip skip) {
-    a = team_sum<TEAM>(a, sh.sum);
+    a = team_sum<TEAM, ENT>(a, sh.sum);
     if (!again) {
         if (plain_sum(a)) return Stat{a.r, a.s, a.w, false};
         if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat{0.f, 0.f, 0.f, false};
@@ -753,13 +753,13 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
     Stat st;
     float l2 = 0.f;
     if constexpr (PART) {
-        a = team_sum<TEAM>(a, sh.sum);
+        a = team_sum<TEAM, true>(a, sh.sum);
         const bool plain = plain_sum(a);
         const float all = plain ? 0.f : team_max<TEAM>(mx, sh.f);
         st.wide = !plain && all != -INFINITY;
         if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, plain ? a.w : 0.f, st.wide);
     } else {
-        st = row_stat<T, TEAM>(a, mx, x, mk, V, R.c, sh, false, [](int) { return false; });
+        st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, false, [](int) { return false; });
         l2 = lg2(st.s);
         if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
     }
@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
         const Soft v = soft_pass<T, 256>(x, mk, R.V, R.c, sh.soft, [](int) { return false; });
         st = Stat{v.m, v.s, v.w, true};
     } else {
-        a = team_sum<256>(a, sh.sum);
+        a = team_sum<256, true>(a, sh.sum);
         st = Stat{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
     }
     const float l2 = lg2(st.s);
@@ -1288,7 +1288,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         Best none{-INFINITY, 0};
         row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
-    const Stat v = row_stat<T, TEAM>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
+    const Stat v = row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
     if (tid < 64) {
         const Row o = row_coefficients(R, Te, E, h, v, repeats);
         if (tid == 0) {
@@ -1373,7 +1373,7 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
     float mx = -INFINITY;
     Best none{-INFINITY, 0};
     row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0}, r < O.keep);
-    a = team_sum<256>(a, sh.sum);
+    a = team_sum<256, false>(a, sh.sum);
     const bool plain = plain_sum(a);
     const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
     if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, 0.f, again);
@@ -1396,6 +1396,9 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     Entries& E = Es[team_in_block<TEAM>()];
     EntryHead h;
     bool repeats = false;
+    float4 part{-FAR, 0.f, 0.f, 0.f};  // ahead of the entries: their loads wait for each other
+    if constexpr (JOIN)
+        if (tid < P.n) part = P.part[r * P.n + tid];
     if (tid < 64) {
         h = load_entries<T>(E, fetch_entries<T>(Te, r, R.V, x, mk), Te, R.c);
         if constexpr (JOIN) repeats = find_repeats(E, Te.k);
@@ -1403,9 +1406,9 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     Row o;
     if constexpr (JOIN) {
         if (tid < 64) {
-            Sum a{-FAR, 0.f, 0.f};
-            bool again = Te.rest && h.far;
-            for (int i = tid; i < P.n; i += 64) {
+            Sum a{part.x, part.y, 0.f};
+            bool again = (Te.rest && h.far) || part.w != 0.f;
+            for (int i = tid + 64; i < P.n; i += 64) {
                 const float4 p = P.part[r * P.n + i];
                 const float m = fmaxf(a.r, p.x);
                 const Sum b = move_sum(Sum{p.x, p.y, 0.f}, m);
@@ -1413,7 +1416,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
                 a.s += b.s;
                 again |= p.w != 0.f;
             }
-            a = team_sum<64>(a, nullptr);
+            a = team_sum<64, false>(a, nullptr);
             again = __ballot(again) != 0;
             if (tid == 0) joined = make_float4(a.s > 0.f ? a.r : 0.f, a.s, 0.f, again);
         }
@@ -1432,25 +1435,27 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
         if (tid < 64) {
             o = row_coefficients(R, Te, E, h, v, repeats);
             if (tid == 0) row = o;
-            if (blockIdx.z == 0) {
-                const float kl = row_kl(R, Te, E, h, o);
-                if (tid == 0) {
-                    O.row_loss[r] = kl;
-                    if (O.stats) ((Row*)O.stats)[r] = o;
-                }
-            }
         }
-        if (!O.dx) return;
         __syncthreads();
         o = row;
     } else {
         o = ((const Row*)O.stats)[r];
     }
-    const float g = row_weight(R, O, r);
-    T* d = (T*)O.dx + r * (long long)R.V + from;
-    write_outside<T, TEAM, MASK>(R, o, g, x + from, MASK ? mk + from : nullptr, d, V, O.nt);
-    team_sync<TEAM>();
-    write_entries<T, TEAM>(R, Te, E, o, g, MASK ? mk + from : nullptr, d, from, V);
+    if (!JOIN || O.dx) {
+        const float g = row_weight(R, O, r);
+        T* d = (T*)O.dx + r * (long long)R.V + from;
+        write_outside<T, TEAM, MASK>(R, o, g, x + from, MASK ? mk + from : nullptr, d, V, O.nt);
+        team_sync<TEAM>();
+        write_entries<T, TEAM>(R, Te, E, o, g, MASK ? mk + from : nullptr, d, from, V);
+    }
+    if constexpr (JOIN)
+        if (blockIdx.z == 0 && tid < 64) {
+            const float kl = row_kl(R, Te, E, h, o);
+            if (tid == 0) {
+                O.row_loss[r] = kl;
+                if (O.stats) ((Row*)O.stats)[r] = o;
+            }
+        }
 }
 
 // out = scale sum_r w_r loss_r in a fixed order, f64
