@@ -187,20 +187,65 @@ __device__ __forceinline__ void apply_mask(const uint8_t* mk, float* f) {
     for (int i = 0; i < VN<T>; ++i) f[i] = b[i] ? f[i] : -INFINITY;
 }
 
+// ln s in f64, s >= 0: s = 2^e f, f in [0.75, 1.5), ln f = 2 atanh(v), v = (f - 1) / (f + 1), |v| <= 0.2, by its power
+// series to v^15 (what is left is under 2e-13)
+__device__ __forceinline__ double ln_f64(double s) {
+    if (!(s > 0.0 && s < INFINITY)) return s == 0.0 ? -INFINITY : s == INFINITY ? INFINITY : NAN;
+    int e = __builtin_amdgcn_frexp_exp(s);
+    double f = __builtin_amdgcn_frexp_mant(s);
+    if (f < 0.75) {
+        f *= 2.0;
+        --e;
+    }
+    const double v = (f - 1.0) / (f + 1.0), w = v * v;
+    double t = 1.0 / 15;
+    t = t * w + 1.0 / 13;
+    t = t * w + 1.0 / 11;
+    t = t * w + 1.0 / 9;
+    t = t * w + 1.0 / 7;
+    t = t * w + 1.0 / 5;
+    t = t * w + 1.0 / 3;
+    t = t * w + 1.0;
+    return 0.69314718055994530942 * e + 2.0 * v * t;
+}
+// e^t in f64: t = n ln 2 + z, |z| <= 0.35, its power series to z^9 (what is left is under 1e-11 of it)
+__device__ __forceinline__ double exp_f64(double t) {
+    const double n = fmin(fmax(rint(t * 1.4426950408889634074), -2000.0), 2000.0);
+    const double z = __builtin_fma(n, -0.69314718055994530942, t);
+    double p = 1.0 / 362880;
+    p = p * z + 1.0 / 40320;
+    p = p * z + 1.0 / 5040;
+    p = p * z + 1.0 / 720;
+    p = p * z + 1.0 / 120;
+    p = p * z + 1.0 / 24;
+    p = p * z + 1.0 / 6;
+    p = p * z + 0.5;
+    p = p * z + 1.0;
+    p = p * z + 1.0;
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
+
 // ---- softmax statistics -------------------------------------------------------------------------
 // s = sum 2^u, w = sum u 2^u with u = x c - r and r a whole number near max x c: moving a sum to another r is exact
 // (a power of two), and x c - r is one rounding.  r follows the maximum lazily (u <= 8.5), and starts at -2^100 with
 // an empty sum.  Where |x c| passes 2^100 (the type's lowest value in f32 and bf16) or a logit is no number, the row
 // is done again by `Soft` below, with u = (x - m) c.
+// ENT: f32 sums with the entropy's; else s alone, in f64 beyond a thread's 16 or 32 terms (a KL is a difference of
+// near values: what s is off by comes to twenty times that of it).
+template <bool ENT>
 struct Sum {
-    float r, s, w;
+    float r;
+    std::conditional_t<ENT, float, double> s;
+    float w;
 };
+__device__ __forceinline__ float scale2(float x, int k) { return __builtin_amdgcn_ldexpf(x, k); }
+__device__ __forceinline__ double scale2(double x, int k) { return __builtin_amdgcn_ldexp(x, k); }
 template <bool ENT, int N>
-__device__ __forceinline__ void sum_group(Sum& a, const float* x, float gm, float c) {
+__device__ __forceinline__ void sum_group(Sum<ENT>& a, const float* x, float gm, float c) {
     if (__builtin_fmaf(gm, c, -a.r) > 8.f) {
         const float r = rintf(gm * c), d = a.r - r;
-        if constexpr (ENT) a.w = __builtin_amdgcn_ldexpf(__builtin_fmaf(d, a.s, a.w), (int)fmaxf(d, -4096.f));
-        a.s = __builtin_amdgcn_ldexpf(a.s, (int)fmaxf(d, -4096.f));
+        if constexpr (ENT) a.w = scale2(__builtin_fmaf(d, a.s, a.w), (int)fmaxf(d, -4096.f));
+        a.s = scale2(a.s, (int)fmaxf(d, -4096.f));
         a.r = r;
     }
     float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
@@ -218,13 +263,15 @@ __device__ __forceinline__ void sum_group(Sum& a, const float* x, float gm, floa
     a.s += s0 + s1;
     if constexpr (ENT) a.w += w0 + w1;
 }
-__device__ __forceinline__ Sum move_sum(Sum a, float r) {  // to a reference r >= a.r
+template <bool ENT>
+__device__ __forceinline__ Sum<ENT> move_sum(Sum<ENT> a, float r) {  // to a reference r >= a.r
     const float d = a.r - r;
     const int k = (int)fmaxf(d, -4096.f);
-    return Sum{r, __builtin_amdgcn_ldexpf(a.s, k), __builtin_amdgcn_ldexpf(__builtin_fmaf(d, a.s, a.w), k)};
+    if constexpr (ENT) a.w = scale2(__builtin_fmaf(d, a.s, a.w), k);
+    return Sum<ENT>{r, scale2(a.s, k), a.w};
 }
 template <int TEAM, bool ENT>
-__device__ __forceinline__ Sum team_sum(Sum a, Sum* sh) {
+__device__ __forceinline__ Sum<ENT> team_sum(Sum<ENT> a, Sum<ENT>* sh) {
     a = move_sum(a, wave_max(a.r));
     a.s = wave_sum(a.s);
     if constexpr (ENT) a.w = wave_sum(a.w);
@@ -235,10 +282,10 @@ __device__ __forceinline__ Sum team_sum(Sum a, Sum* sh) {
         float r = sh[0].r;
 #pragma unroll
         for (int i = 1; i < W; ++i) r = fmaxf(r, sh[i].r);
-        a = Sum{r, 0.f, 0.f};
+        a = Sum<ENT>{r, 0, 0.f};
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const Sum b = move_sum(sh[i], r);
+            const Sum<ENT> b = move_sum(sh[i], r);
             a.s += b.s;
             a.w += b.w;
         }
@@ -289,21 +336,25 @@ __device__ Soft team_soft(Soft v, float c, Soft* sh) {
 }
 
 // A row's statistics as the gradients use them: u = x c - ref, or (x - ref) c on a wide row; p = 2^(u - l2)
+template <bool ENT>
 struct Stat {
-    float ref, s, w;
+    float ref;
+    std::conditional_t<ENT, float, double> s;
+    float w;
     bool wide;
 };
 __device__ __forceinline__ float u_of(float x, float ref, bool wide, float c) {
     return wide ? (x - ref) * c : __builtin_fmaf(x, c, -ref);
 }
 // the log-probability of a logit, l2 = log2 of the row's sum
-__device__ __forceinline__ float logp_of(float x, const Stat& st, float l2, float c, float invT) {
+__device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2, float c, float invT) {
     if (st.wide) return (x - st.ref) * invT - LN2 * l2;
     if (fabsf(x) > 1e30f) return x * invT - LN2 * (st.ref + l2);  // x c may pass f32 where x / T does not
     return LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
 }
 // is this sum a row's (some probability, all numbers)?  An empty one is a row without a legal action, or a wide one.
-__device__ __forceinline__ bool plain_sum(const Sum& a) { return a.s > 0.f && a.s < INFINITY; }
+template <bool ENT>
+__device__ __forceinline__ bool plain_sum(const Sum<ENT>& a) { return a.s > 0.f && a.s < INFINITY; }
 
 // order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {
@@ -316,29 +367,6 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
     return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
 }
 __device__ __forceinline__ unsigned key_index(unsigned long long key) { return 0xFFFFFFFFu - (unsigned)key; }
-
-// ln s in f64 for f32 s > 0: s = 2^e f, f in [0.75, 1.5), ln f = 2 atanh(u), u = (f - 1) / (f + 1), |u| <= 0.2,
-// by its power series to u^15 (what is left is under 2e-13)
-__device__ __forceinline__ double ln_f64(float s) {
-    if (!(s > 0.f && s < INFINITY)) return s == 0.f ? -INFINITY : s == INFINITY ? INFINITY : NAN;
-    int e;
-    float f = frexpf(s, &e);
-    if (f < 0.75f) {
-        f *= 2.f;
-        --e;
-    }
-    const double u = ((double)f - 1.0) / ((double)f + 1.0), w = u * u;
-    double t = 1.0 / 15;
-    t = t * w + 1.0 / 13;
-    t = t * w + 1.0 / 11;
-    t = t * w + 1.0 / 9;
-    t = t * w + 1.0 / 7;
-    t = t * w + 1.0 / 5;
-    t = t * w + 1.0 / 3;
-    t = t * w + 1.0;
-    return 0.69314718055994530942 * e + 2.0 * u * t;
-}
-
 
 // ---- one pass over a row --------------------------------------------------------------------------
 // GROUP vectors of a thread at once: loads first, then the group's maximum, then its exponentials.
@@ -370,7 +398,7 @@ struct NoEdit {
 };
 
 template <class T, int TEAM, bool MASK, bool ENT, bool TOP, bool NT, class Edit>
-__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx, Best& best,
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum<ENT>& a, float& mx, Best& best,
                                          float* gmax, const Edit& edit) {
     constexpr int N = VN<T>;
     const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
@@ -434,7 +462,7 @@ __device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, f
     if (nvec * N < V) sum_group<ENT, 2>(a, f, f[0], c);
 }
 template <class T, int TEAM, bool MASK, bool ENT, bool TOP, class Edit>
-__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum& a, float& mx,
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum<ENT>& a, float& mx,
                                          Best& best, float* gmax, const Edit& edit, bool nt) {
     if (nt)  // the same for the whole team
         row_pass<T, TEAM, MASK, ENT, TOP, true>(x, mk, V, c, a, mx, best, gmax, edit);
@@ -465,23 +493,24 @@ __device__ __forceinline__ float team_max(float x, float* sh) {
     return x;
 }
 
+template <bool ENT>
 union Shared {  // one reduction at a time
-    Sum sum[16];
+    Sum<ENT> sum[16];
     Soft soft[16];
     float f[16];
 };
 
 // a row's statistics from its pass: as they are, or by the element-wise pass; an empty row has s = 0
 template <class T, int TEAM, bool ENT, class Skip>
-__device__ __forceinline__ Stat row_stat(Sum a, float mx, const T* x, const uint8_t* mk, int V, float c, Shared& sh,
-                                         bool again, Skip skip) {
+__device__ __forceinline__ Stat<ENT> row_stat(Sum<ENT> a, float mx, const T* x, const uint8_t* mk, int V, float c,
+                                              Shared<ENT>& sh, bool again, Skip skip) {
     a = team_sum<TEAM, ENT>(a, sh.sum);
     if (!again) {
-        if (plain_sum(a)) return Stat{a.r, a.s, a.w, false};
-        if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat{0.f, 0.f, 0.f, false};
+        if (plain_sum(a)) return Stat<ENT>{a.r, a.s, a.w, false};
+        if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat<ENT>{0.f, 0, 0.f, false};
     }
     const Soft v = soft_pass<T, TEAM>(x, mk, V, c, sh.soft, skip);
-    return Stat{v.m, v.s, v.w, true};
+    return Stat<ENT>{v.m, v.s, v.w, true};
 }
 
 // ---- the k largest of a row -----------------------------------------------------------------------
@@ -701,7 +730,7 @@ __device__ __forceinline__ long long action_of(const LogprobsOut& O, long long r
 }
 
 template <class T>
-__device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat& st, float l2,
+__device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat<true>& st, float l2,
                                           long long act, const T* x, const uint8_t* mk) {
     const bool empty = st.s == 0.f;
     const float H = empty ? 0.f : LN2 * (l2 - st.w / st.s);
@@ -729,7 +758,7 @@ template <class T, int TEAM, bool MASK, bool TOP, bool PART>
 __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, LogprobsOut O, Split P) {
     extern __shared__ float gmax_all[];
     constexpr int TEAMS = block_of<TEAM> / TEAM;
-    __shared__ Shared sh;
+    __shared__ Shared<true> sh;
     __shared__ TopShare<TEAM> tops[TOP ? TEAMS : 1];
     const long long r = team_row<TEAM>();
     if (r >= R.rows) return;
@@ -746,11 +775,11 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
     float* gmax = gmax_all + team_in_block<TEAM>() * ((V / VN<T> + TEAM * GROUP - 1) / (TEAM * GROUP) + 1) * TEAM;
     long long act = -1;
     if constexpr (!PART) act = action_of(O, r);
-    Sum a{-FAR, 0.f, 0.f};
+    Sum<true> a{-FAR, 0.f, 0.f};
     float mx = -INFINITY;
     Best best{-INFINITY, 0};
     row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{}, r < O.keep);
-    Stat st;
+    Stat<true> st;
     float l2 = 0.f;
     if constexpr (PART) {
         a = team_sum<TEAM, true>(a, sh.sum);
@@ -782,7 +811,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
 // the parts of a row joined
 template <class T, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut O, Split P) {
-    __shared__ Shared sh;
+    __shared__ Shared<true> sh;
     __shared__ TopShare<256> S;
     const long long r = block_row();
     if (r >= R.rows) return;
@@ -790,12 +819,12 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
     const uint8_t* mk = mask_ptr(R, r);
     const int tid = threadIdx.x;
     const long long act = action_of(O, r);
-    Sum a{-FAR, 0.f, 0.f};
+    Sum<true> a{-FAR, 0.f, 0.f};
     bool again = false;
     for (int i = tid; i < P.n; i += 256) {
         const float4 p = P.part[r * P.n + i];
         const float m = fmaxf(a.r, p.x);
-        const Sum b = move_sum(Sum{p.x, p.y, p.z}, m);
+        const Sum<true> b = move_sum(Sum<true>{p.x, p.y, p.z}, m);
         a = move_sum(a, m);
         a.s += b.s;
         a.w += b.w;
@@ -809,13 +838,13 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
         for (int i = tid; i < nk; i += 256) best = best > keys[i] ? best : keys[i];
     }
     again = __syncthreads_or(again);
-    Stat st;
+    Stat<true> st;
     if (again) {
         const Soft v = soft_pass<T, 256>(x, mk, R.V, R.c, sh.soft, [](int) { return false; });
-        st = Stat{v.m, v.s, v.w, true};
+        st = Stat<true>{v.m, v.s, v.w, true};
     } else {
         a = team_sum<256, true>(a, sh.sum);
-        st = Stat{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
+        st = Stat<true>{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
     }
     const float l2 = lg2(st.s);
     if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
@@ -937,13 +966,14 @@ struct Teacher {
 // a row's teacher entries: ids (-1: none), the student's logits there (illegal: -inf), t, q = exp(t - tm) / qs (rest:
 // exp t); first: no earlier entry has the same id
 struct Entries {
+    double q[TOP_MAX];
     int id[TOP_MAX];
-    float x[TOP_MAX], t[TOP_MAX], q[TOP_MAX];
+    float x[TOP_MAX], t[TOP_MAX];
     bool first[TOP_MAX];
 };
 struct EntryHead {
-    double Q;  // sum q
-    float tm, qs;
+    double qs;  // the entries' sum (rest: of q)
+    float tm;
     bool any, far;  // far: a student's logit that Sum does not hold
 };
 struct EntryRegs {  // as loaded, an entry or two a lane
@@ -999,35 +1029,28 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
     h.tm = wave_max(h.tm);
     h.any = h.tm != -INFINITY;
     if (Te.rest || !h.any) h.tm = 0.f;
-    float q[2];
-    h.qs = 0.f;
+    double q[2] = {0.0, 0.0};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        q[u] = 0.f;
         if (64 * u >= Te.k) continue;
-        q[u] = id[u] >= 0 ? expf(e.t[u] - h.tm) : 0.f;
-        h.qs += q[u];
+        if (id[u] >= 0) q[u] = exp_f64((double)e.t[u] - (double)h.tm);
     }
-    h.qs = wave_sum(h.qs);
-    const float iq = Te.rest || !h.any ? 1.f : 1.f / h.qs;
-    h.Q = 0.0;
+    h.qs = wave_sum(q[0] + q[1]);
+    const double iq = Te.rest || !h.any ? 1.0 : 1.0 / h.qs;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
         if (64 * u >= Te.k) continue;
-        q[u] *= iq;
-        h.Q += q[u];
         if (j < Te.k) {
             const float xj = id[u] >= 0 && e.legal[u] ? e.x[u] : -INFINITY;
             far |= xj != -INFINITY && !(fabsf(xj * c) < FAR);
             E.id[j] = id[u];
             E.t[j] = e.t[u];
             E.x[j] = xj;
-            E.q[j] = q[u];
+            E.q[j] = q[u] * iq;
             E.first[j] = true;
         }
     }
-    if (Te.rest) h.Q = wave_sum(h.Q);  // else it is 1
     h.far = __ballot(far) != 0;
     team_sync<64>();
     return h;
@@ -1057,14 +1080,17 @@ struct Row {  // what the gradient needs of a row: p(x, ref, s) = 2^u(x, ref) / 
     float ra, sa, a;  // dx = (a p(x, ra, sa) - q) w / T at the entries
     float wide, repeats;
 };
+struct RowSums {  // so, sa as summed, for the loss
+    double so, sa;
+};
 
 // a row's coefficients, by one wave, from the student's statistics v over all legal actions outside the entries
 // (rest) or over all (else)
 __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
-                                                const Stat& v, bool repeats) {
+                                                const Stat<false>& v, bool repeats, RowSums* sums) {
     const int lane = threadIdx.x & 63;
-    Stat all = v;
-    float po = 1.f;  // the student's mass outside the entries
+    Stat<false> all = v;
+    double po = 1.0;  // the student's mass outside the entries
     if (Te.rest) {
         float xj[2], mx = -INFINITY;
 #pragma unroll
@@ -1075,43 +1101,44 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
             mx = nmax(mx, xj[u]);
         }
         mx = wave_max(mx);
-        Stat e{0.f, 0.f, 0.f, v.wide};
+        Stat<false> e{0.f, 0.0, 0.f, v.wide};
         if (mx != -INFINITY) {
             e.ref = v.wide ? mx : rintf(mx * R.c);
-            e.s = wave_sum(ex2(u_of(xj[0], e.ref, v.wide, R.c)) + ex2(u_of(xj[1], e.ref, v.wide, R.c)));
+            e.s = wave_sum((double)ex2(u_of(xj[0], e.ref, v.wide, R.c)) + (double)ex2(u_of(xj[1], e.ref, v.wide, R.c)));
         }
-        po = v.s != 0.f ? 1.f : 0.f;
-        if (e.s != 0.f && v.s != 0.f) {
+        po = v.s != 0.0 ? 1.0 : 0.0;
+        if (e.s != 0.0 && v.s != 0.0) {
             all.ref = nmax(e.ref, v.ref);
-            const float se = e.s * ex2(v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref);
-            const float sv = v.s * ex2(v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref);
+            const double se = e.s * (double)ex2(v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref);
+            const double sv = v.s * (double)ex2(v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref);
             all.s = se + sv;
             po = sv / all.s;
-        } else if (e.s != 0.f) {
+        } else if (e.s != 0.0) {
             all = e;
         }
     }
-    double S = Te.rest ? h.Q : 1.0, qr = 0.0;
-    if (Te.rest && v.s != 0.f) {
-        qr = 1.0 - h.Q;
+    double S = Te.rest ? h.qs : 1.0, qr = 0.0;
+    if (Te.rest && v.s != 0.0) {
+        qr = 1.0 - h.qs;
         if (qr < 0.0) qr = 0.0;
         S += qr;
     }
-    if (!h.any || all.s == 0.f) S = 0.0, qr = 0.0;
-    return Row{v.ref, v.s, (float)(S * (double)po - qr), all.ref, all.s, (float)S, v.wide ? 1.f : 0.f,
+    if (!h.any || all.s == 0.0) S = 0.0, qr = 0.0;
+    *sums = RowSums{v.s, all.s};
+    return Row{v.ref, (float)v.s, (float)(S * po - qr), all.ref, (float)all.s, (float)S, v.wide ? 1.f : 0.f,
                repeats ? 1.f : 0.f};
 }
 
 // the row's loss, by one wave, its terms in f64
 __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const Entries& E, const EntryHead& h,
-                                        const Row& o) {
-    if (!h.any || o.sa == 0.f) return 0.f;
+                                        const Row& o, const RowSums& sums) {
+    if (!h.any || sums.sa == 0.0) return 0.f;
     const int lane = threadIdx.x & 63;
     const bool wide = o.wide != 0.f;
     const double cd = R.c, ln2 = 0.69314718055994530942;
     // the row's logarithms at once, one a lane: of the sums over all and outside, of the entries' sum, of what is left
-    const double qr = 1.0 - h.Q;
-    const double ln = ln_f64(lane == 0 ? o.sa : lane == 1 ? o.so : lane == 2 ? h.qs : (float)qr);
+    const double qr = 1.0 - h.qs;
+    const double ln = ln_f64(lane == 0 ? sums.sa : lane == 1 ? sums.so : lane == 2 ? h.qs : qr);
     const double lns = lane_of(ln, 0), lnq = Te.rest ? 0.0 : lane_of(ln, 2);
     double loss = 0.0;
 #pragma unroll
@@ -1124,7 +1151,7 @@ __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const 
         if (q > 0.0 || q != q) loss += q * (lq - (uj * ln2 - lns));
     }
     loss = wave_sum(loss);
-    if (Te.rest && o.so != 0.f) {
+    if (Te.rest && sums.so != 0.0) {
         const double d = wide ? ((double)o.ro - (double)o.ra) * cd : (double)o.ro - (double)o.ra;
         if (!(qr <= 0.0)) loss += qr * (lane_of(ln, 3) - (d * ln2 + lane_of(ln, 1) - lns));
     }
@@ -1165,10 +1192,11 @@ __device__ __forceinline__ void write_entries(const Rows& R, const Teacher& Te, 
     for (int j = team_tid<TEAM>(); j < Te.k; j += TEAM) {
         const int id = E.id[j], i = id - from;
         if (id < 0 || i < 0 || i >= V || (mk && !mk[i])) continue;
-        float q = E.q[j];
+        float q = (float)E.q[j];
         if (o.repeats != 0.f) {  // the same index twice: its entries' probabilities add
-            q = 0.f;
-            for (int e = 0; e < Te.k; ++e) q += E.id[e] == id ? E.q[e] : 0.f;
+            double all = 0.0;
+            for (int e = 0; e < Te.k; ++e) all += E.id[e] == id ? E.q[e] : 0.0;
+            q = (float)all;
         }
         const float p = ex2(u_of(E.x[j], o.ra, o.wide != 0.f, R.c)) * (o.a / o.sa);
         d[i] = (T)(o.a == 0.f ? 0.f : (p - q) * g);  // a = 0: a row without a legal action
@@ -1207,9 +1235,10 @@ __global__ __launch_bounds__(block_of<TEAM>) __attribute__((amdgpu_waves_per_eu(
 void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     extern __shared__ unsigned bits_all[];
     constexpr int TEAMS = block_of<TEAM> / TEAM, N = VN<T>;
-    __shared__ Shared sh;
+    __shared__ Shared<false> sh;
     __shared__ Entries Es[TEAMS];
     __shared__ Row rows[TEAMS];
+    __shared__ RowSums sums[TEAMS];
     __shared__ bool fars[TEAMS];
     const long long r = team_row<TEAM>();
     if (r >= R.rows) return;
@@ -1253,7 +1282,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         team_sync<TEAM>();
     }
     const SkipBits<T> skip{bits, Te.rest != 0};
-    Sum a{-FAR, 0.f, 0.f};
+    Sum<false> a{-FAR, 0.0, 0.f};
     float mx = -INFINITY;
     if constexpr (NV > 0) {
 #pragma unroll
@@ -1288,18 +1317,20 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         Best none{-INFINITY, 0};
         row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
-    const Stat v = row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
+    const Stat<false> v = row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
     if (tid < 64) {
-        const Row o = row_coefficients(R, Te, E, h, v, repeats);
+        RowSums both;
+        const Row o = row_coefficients(R, Te, E, h, v, repeats, &both);
         if (tid == 0) {
             rows[mine] = o;
+            sums[mine] = both;
             if (O.stats) ((Row*)O.stats)[r] = o;
         }
     }
     team_sync<TEAM>();
     auto loss = [&] {
         if (tid < 64) {
-            const float kl = row_kl(R, Te, E, h, rows[mine]);
+            const float kl = row_kl(R, Te, E, h, rows[mine], sums[mine]);
             if (tid == 0) O.row_loss[r] = kl;
         }
     };
@@ -1344,11 +1375,15 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     loss();  // last: the other waves do not wait for it
 }
 
-// a part of a row of few rows: its statistics outside the entries
+// a part of a row of few rows: its statistics outside the entries, as (r, s in two words, 1 if the row is a wide one)
+__device__ __forceinline__ Sum<false> part_sum(float4 p) {
+    const unsigned long long w = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.y);
+    return Sum<false>{p.x, __longlong_as_double((long long)w), 0.f};
+}
 template <class T, bool MASK>
 __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, DistillOut O, Split P) {
     extern __shared__ unsigned bits[];
-    __shared__ Shared sh;
+    __shared__ Shared<false> sh;
     const long long r = block_row();
     if (r >= R.rows) return;
     const int tid = threadIdx.x, from = blockIdx.z * P.len, V = R.V - from < P.len ? R.V - from : P.len;
@@ -1369,14 +1404,18 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
         set_bit(bits, id, from, V);
         __syncthreads();
     }
-    Sum a{-FAR, 0.f, 0.f};
+    Sum<false> a{-FAR, 0.0, 0.f};
     float mx = -INFINITY;
     Best none{-INFINITY, 0};
     row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0}, r < O.keep);
     a = team_sum<256, false>(a, sh.sum);
     const bool plain = plain_sum(a);
     const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
-    if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, 0.f, again);
+    if (tid == 0) {
+        const unsigned long long w = (unsigned long long)__double_as_longlong(plain ? a.s : 0.0);
+        P.part[r * P.n + blockIdx.z] =
+            make_float4(a.r, __uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)), again);
+    }
 }
 
 // a row or a part of it of the gradient, from the row's statistics (stats) or from its parts (JOIN: then the first
@@ -1384,10 +1423,10 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
 template <class T, int TEAM, bool MASK, bool JOIN>
 __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Teacher Te, DistillOut O, Split P, int len) {
     constexpr int TEAMS = block_of<TEAM> / TEAM;
-    __shared__ Shared sh;
+    __shared__ Shared<false> sh;
     __shared__ Entries Es[TEAMS];
     __shared__ Row row;
-    __shared__ float4 joined;
+    __shared__ Stat<false> joined;
     const long long r = R.rows - 1 - team_row<TEAM>();
     if (r < 0) return;
     const int tid = team_tid<TEAM>(), from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
@@ -1404,25 +1443,26 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
         if constexpr (JOIN) repeats = find_repeats(E, Te.k);
     }
     Row o;
+    RowSums sums;
     if constexpr (JOIN) {
         if (tid < 64) {
-            Sum a{part.x, part.y, 0.f};
+            Sum<false> a = part_sum(part);
             bool again = (Te.rest && h.far) || part.w != 0.f;
             for (int i = tid + 64; i < P.n; i += 64) {
                 const float4 p = P.part[r * P.n + i];
                 const float m = fmaxf(a.r, p.x);
-                const Sum b = move_sum(Sum{p.x, p.y, 0.f}, m);
+                const Sum<false> b = move_sum(part_sum(p), m);
                 a = move_sum(a, m);
                 a.s += b.s;
                 again |= p.w != 0.f;
             }
             a = team_sum<64, false>(a, nullptr);
             again = __ballot(again) != 0;
-            if (tid == 0) joined = make_float4(a.s > 0.f ? a.r : 0.f, a.s, 0.f, again);
+            if (tid == 0) joined = Stat<false>{a.s > 0.0 ? a.r : 0.f, a.s, 0.f, again};
         }
         __syncthreads();
-        Stat v{joined.x, joined.y, 0.f, false};
-        if (joined.w != 0.f) {
+        Stat<false> v = joined;
+        if (v.wide) {
             const bool rest = Te.rest;
             const int k = Te.k;
             const Soft s = soft_pass<T, TEAM>(x, mk, R.V, R.c, sh.soft, [&](int i) {
@@ -1430,10 +1470,10 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
                     if (E.id[j] == i) return true;
                 return false;
             });
-            v = Stat{s.m, s.s, 0.f, true};
+            v = Stat<false>{s.m, s.s, 0.f, true};
         }
         if (tid < 64) {
-            o = row_coefficients(R, Te, E, h, v, repeats);
+            o = row_coefficients(R, Te, E, h, v, repeats, &sums);
             if (tid == 0) row = o;
         }
         __syncthreads();
@@ -1450,7 +1490,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     }
     if constexpr (JOIN)
         if (blockIdx.z == 0 && tid < 64) {
-            const float kl = row_kl(R, Te, E, h, o);
+            const float kl = row_kl(R, Te, E, h, o, sums);
             if (tid == 0) {
                 O.row_loss[r] = kl;
                 if (O.stats) ((Row*)O.stats)[r] = o;

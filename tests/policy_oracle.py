@@ -1,4 +1,4 @@
-"""The policy operators' definitions in 64 bits (plain torch on the CPU), and how far f32 kernels may be off.
+"""The policy operators' definitions in 64 bits (plain torch, on the device of the logits), and how far f32 kernels may be off.
 
 Units: h = 2^-24, half a step of f32.  A row's sum of V exponentials, each thread adding at most V / 64 of
 them before a tree, is off by at most (V / 64 + 16) h of itself; an exponential 2^u by its instruction's 2 h and by
@@ -17,9 +17,9 @@ TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 
 
 def softmax64(x, mask, T):
     """x [n, V] any type -> z = x / T (illegal: -inf), lse, logp, p in f64; a row without a legal action: p = 0"""
-    z = x.detach().cpu().double() / T
+    z = x.detach().double() / T
     if mask is not None:
-        z = torch.where(mask.cpu().bool(), z, torch.full_like(z, -math.inf))
+        z = torch.where(mask.to(x.device).bool(), z, torch.full_like(z, -math.inf))
     m = z.max(1, keepdim=True).values
     none = m[:, 0] == -math.inf
     # from the maximum, not from lse: next to the type's lowest value the logarithm of the sum is lost even in f64
@@ -49,14 +49,14 @@ def logprobs(x, actions, mask, T, top):
     m = z.max(1).values
     r = {"lse": (lse, sl + 3 * H * m.abs().nan_to_num(0, 0, 0)), "entropy": (ent, 2 * sl * (2 + eu))}
     if actions is not None:
-        a = actions.cpu().long().reshape(-1)
+        a = actions.to(x.device).long().reshape(-1)
         inside = (a >= 0) & (a < V)
-        la = logp[torch.arange(n), a.clamp(0, V - 1)]
+        la = logp.gather(1, a.clamp(0, V - 1)[:, None])[:, 0]
         la = torch.where(inside, la, torch.zeros_like(la))
-        za = (z[torch.arange(n), a.clamp(0, V - 1)] - m).abs().nan_to_num(0, 0, 0)
+        za = (z.gather(1, a.clamp(0, V - 1)[:, None])[:, 0] - m).abs().nan_to_num(0, 0, 0)
         r["logp"] = (la, sl + 4 * H * za)
     if top:
-        key = x.detach().cpu().float()
+        key = x.detach().float()
         key = torch.where(torch.isfinite(z) | (z == math.inf), key, torch.full_like(key, -math.inf))
         v, i = torch.sort(key, dim=1, descending=True, stable=True)
         v, i = v[:, :top], i[:, :top]
@@ -74,16 +74,17 @@ def logprobs_grad(x, actions, mask, T, g1, g2, g3):
     z, lse, logp, p = softmax64(x, mask, T)
     ent = -torch.special.xlogy(p, p).sum(1, keepdim=True)
     sl, eu = row_slack(z, p)
-    g1, g2, g3 = (torch.zeros(n, 1, dtype=torch.float64) if g is None else g.cpu().double().reshape(n, 1)
+    g1, g2, g3 = (torch.zeros(n, 1, dtype=torch.float64, device=x.device) if g is None else
+                  g.to(x.device).double().reshape(n, 1)
                   for g in (g1, g2, g3))
-    hot = torch.zeros(n, V, dtype=torch.float64)
+    hot = torch.zeros(n, V, dtype=torch.float64, device=x.device)
     if actions is not None:
-        a = actions.cpu().long().reshape(-1)
+        a = actions.to(x.device).long().reshape(-1)
         inside = (a >= 0) & (a < V) & (lse > -math.inf)
         if mask is not None:
-            inside &= mask.cpu().bool()[torch.arange(n), a.clamp(0, V - 1)]
+            inside &= mask.to(x.device).bool().gather(1, a.clamp(0, V - 1)[:, None])[:, 0]
         given = (a >= 0) & (a < V)
-        hot[torch.arange(n), a.clamp(0, V - 1)] = inside.double()
+        hot.scatter_(1, a.clamp(0, V - 1)[:, None], inside.double()[:, None])
         g1 = torch.where(given[:, None], g1, torch.zeros_like(g1))
     lp = torch.where(p > 0, logp, torch.zeros_like(logp))
     d = (g1 * (hot - p) + g3 * p - g2 * p * (lp + ent)) / T
@@ -99,8 +100,8 @@ def distill(x, t_logp, t_ids, mask, T, rest):
     k = t_ids.shape[1]
     z, lse, logp, p = softmax64(x, mask, T)
     sl, eu = row_slack(z, p)
-    t = t_logp.detach().cpu().double()
-    ids = t_ids.cpu().long()
+    t = t_logp.detach().to(x.device).double()
+    ids = t_ids.to(x.device).long()
     there = (ids >= 0) & (ids < V) & (t != -math.inf)
     ids = ids.clamp(0, V - 1)
     if rest:
@@ -146,7 +147,7 @@ def distill(x, t_logp, t_ids, mask, T, rest):
     loss = torch.where(nothing, torch.zeros_like(loss), loss)
     tol = tol + H * loss.abs().nan_to_num(0, 0, 0)
     if mask is not None:
-        tgt = torch.where(mask.cpu().bool(), tgt, torch.zeros_like(tgt))
+        tgt = torch.where(mask.to(x.device).bool(), tgt, torch.zeros_like(tgt))
     d = torch.where(nothing[:, None], torch.zeros_like(p), (p * S[:, None] - tgt - rp) / T)
     lpa = torch.where(p > 0, logp, torch.zeros_like(p)).abs()
     dd = p * S[:, None] * (3 * sl[:, None] + 8 * H * (lpa + 2)) + p * dS[:, None] + 16 * H * tgt + dr + \
@@ -161,7 +162,7 @@ def grad_tol(d, dd, w, dtype):
 
 
 def check(got, want, tol, what):
-    got = got.detach().cpu().double().reshape(want.shape)
+    got = got.detach().double().reshape(want.shape)
     same = (got == want) | (torch.isnan(got) & torch.isnan(want))
     off = torch.where(same, torch.zeros_like(want), (got - want).abs())
     bad = ~(same | (off <= tol))

@@ -105,7 +105,7 @@ def _check_logprobs(x, mask, actions, top, T=1.0, grads=True, seed=0):
     for k in ("lse", "entropy", "logp"):
         po.check(getattr(r, k), want[k][0], want[k][1], k)
     if top:
-        assert torch.equal(r.top_ids.cpu().view(n, top), want["top_ids"])
+        assert torch.equal(r.top_ids.cpu().view(n, top), want["top_ids"].cpu())
         po.check(r.top_logp, *want["top_logp"], "top_logp")
     else:
         assert r.top_ids is None and r.top_logp is None
@@ -192,14 +192,14 @@ def _teacher(x, k, mask, seed=0, noise=0.5):
     """(log-probabilities, ids) of a teacher near the student, with missing, doubled and low entries"""
     n, V = x.shape
     g = torch.Generator().manual_seed(seed + 11 * V + k)
-    t = x.detach().cpu().float().clamp(-60, 60) + noise * torch.randn((n, V), generator=g)
+    t = x.detach().float().clamp(-60, 60) + noise * torch.randn((n, V), generator=g).cuda()
     if mask is not None:
-        t = t.masked_fill(~mask.cpu().bool(), -math.inf)
+        t = t.masked_fill(~mask.cuda().bool(), -math.inf)
     v, i = torch.topk(t, min(k, V), dim=1)
     lse = torch.logsumexp(t, 1, keepdim=True)
     v = torch.where(v == -math.inf, v, v - lse)
     i = torch.where(v == -math.inf, -1, i)
-    return v, i
+    return v.cpu(), i.cpu()
 
 
 def _check_distill(x, mask, t, ids, rest, T=1.0, seed=0, t_dtype=torch.float32, i_dtype=torch.int64):
@@ -219,9 +219,9 @@ def _check_distill(x, mask, t, ids, rest, T=1.0, seed=0, t_dtype=torch.float32, 
     assert rows.shape == lead and rows.dtype == torch.float32
     po.check(rows, loss, tol, "row loss")
     g = torch.Generator().manual_seed(seed + 3)
-    w = torch.randn((n,), generator=g)
+    w = torch.randn((n,), generator=g).cuda()
     # the whole and its gradient in one call, weighted by row
-    total, dx = p.distill_loss_grad(x, *args, weight=w.cuda().view(lead), **kw)
+    total, dx = p.distill_loss_grad(x, *args, weight=w.view(lead), **kw)
     w64 = w.double()
     if loss.isfinite().all():
         po.check(total, (loss * w64).sum(), (tol * w64.abs()).sum() + po.H * (loss * w64).sum().abs() + 1e-30, "total")
@@ -229,11 +229,11 @@ def _check_distill(x, mask, t, ids, rest, T=1.0, seed=0, t_dtype=torch.float32, 
     po.check(dx, d * w64[:, None], po.grad_tol(d, dd, w64[:, None], x.dtype), "gradient")
     # through autograd: rows weighted from outside, and the mean
     leaf = x.detach().requires_grad_(True)
-    d1, = torch.autograd.grad(p.distill_loss(leaf, *args, reduction="none", **kw), leaf, w.cuda().view(lead))
+    d1, = torch.autograd.grad(p.distill_loss(leaf, *args, reduction="none", **kw), leaf, w.view(lead))
     po.check(d1, d * w64[:, None], po.grad_tol(d, dd, w64[:, None], x.dtype), "autograd rows")
     mean = p.distill_loss(leaf, *args, **kw)
     d2, = torch.autograd.grad(mean * 3.0, leaf)
-    w3 = torch.full((1, 1), 3.0 / n, dtype=torch.float64)
+    w3 = torch.full((1, 1), 3.0 / n, dtype=torch.float64, device=x.device)
     if loss.isfinite().all():
         po.check(mean, loss.mean(), tol.mean() + po.H * 2 * loss.mean().abs(), "mean")
     po.check(d2, d * w3, po.grad_tol(d, dd, w3, x.dtype), "autograd mean")
@@ -338,6 +338,102 @@ def test_distill_values(values, dtype):
             _check_distill(x, None, t, ids, rest)
 
 
+# enough rows that none is split over blocks: a wave, a block of each size and the rows in registers
+MANY = [(2100, 3001, "f32"), (2100, 4096, "f32"), (2100, 8190, "bf16"), (2100, 1500, "f16"), (130, 2050, "f32"),
+        (130, 8193, "f32"), (130, 9001, "f16"), (130, 16384, "f32"), (130, 20011, "bf16"), (130, 32768, "f16"),
+        (130, 33001, "f32"), (130, 65536, "f32"), (130, 65537, "f32"), (129, 65543, "bf16"), (128, 131072, "f16"),
+        (128, 131073, "bf16")]
+
+
+@pytest.mark.parametrize("n,V,dtype", MANY)
+def test_logprobs_many_rows(n, V, dtype):
+    for kind, top in (("none", 9), ("empty", 40), ("random", 128), ("shared", 0)):
+        if n > 2000 and kind in ("random", "shared"):
+            continue
+        _check_logprobs(_logits(n, V, DT[dtype]), _mask(kind, n, V), _actions(n, V), top, grads=kind in ("none", "empty"))
+
+
+@pytest.mark.parametrize("values", ["ties", "constant", "falling", "rising", "cluster", "stripes", "lowest", "minf"])
+@pytest.mark.parametrize("n,V,dtype", [(130, 3001, "f32"), (130, 20011, "bf16"), (130, 20011, "f32")])
+def test_logprobs_many_rows_values(n, V, dtype, values):
+    x = _logits(n, V, DT[dtype], values=values)
+    for top in (20, 100):
+        _check_logprobs(x, None, _actions(n, V), top, grads=top == 20)
+
+
+@pytest.mark.parametrize("n,V,dtype", MANY)
+def test_distill_many_rows(n, V, dtype):
+    for kind, k, rest in (("none", 33, True), ("empty", 100, True), ("shared", 7, False)):
+        if n > 2000 and kind == "shared":
+            continue
+        x = _logits(n, V, DT[dtype])
+        m = _mask(kind, n, V)
+        t, ids = _teacher(x, k, _full(m, n, V))
+        ids[3, k - 1] = ids[3, 0]
+        if m is not None:
+            x[_full(m, n, V) == 0] = math.nan
+        _check_distill(x, m, t, ids, rest)
+
+
+@pytest.mark.parametrize("values", ["wide", "lowest", "minf", "constant"])
+@pytest.mark.parametrize("n,V,dtype", [(130, 700, "f32"), (130, 12001, "f32"), (130, 20011, "bf16"), (130, 70001, "f16")])
+def test_distill_many_rows_values(n, V, dtype, values):
+    x = _logits(n, V, DT[dtype], values=values)
+    t, ids = _teacher(_logits(n, V, torch.float32, seed=3), 20, x.float() > torch.finfo(DT[dtype]).min)
+    for rest in (False, True):
+        _check_distill(x, None, t, ids, rest)
+
+
+def test_more_rows_than_one_grid_dimension():
+    """2^22 rows of a wave, 2^20 of a block, and a few more."""
+    p = _policy()
+    n = 2 ** 22 + 5
+    x = torch.randn((n, 3), generator=torch.Generator().manual_seed(0)).cuda().requires_grad_(True)
+    a = (torch.arange(n) % 3).cuda()
+    r = p.action_logprobs(x, a, top=1)
+    d, = torch.autograd.grad(r.logp, x, torch.ones(n, device="cuda"))
+    loss, e = p.distill_loss_grad(x, torch.zeros((n, 1), device="cuda"), a[:, None], weight=1.0)
+    for s in (slice(0, 50), slice(2 ** 22 - 25, n)):
+        want = po.logprobs(x[s], a[s], None, 1.0, 1)
+        po.check(r.logp[s], *want["logp"], "logp")
+        assert torch.equal(r.top_ids[s].cpu(), want["top_ids"].cpu())
+        g = torch.ones(x[s].shape[0])
+        po.check(d[s], *po.logprobs_grad(x[s], a[s], None, 1.0, g, None, None), "gradient")
+        po.check(-e[s], *po.logprobs_grad(x[s], a[s], None, 1.0, g, None, None), "distillation of one action")
+    n, V = 2 ** 20 + 3, 8200
+    row = _logits(1, V, torch.bfloat16)
+    r = p.action_logprobs(row.expand(n, V), torch.full((n,), 7, device="cuda"))
+    want = po.logprobs(row, torch.tensor([7]), None, 1.0, 0)
+    po.check(r.logp, want["logp"][0].expand(n), want["logp"][1].expand(n), "logp")
+
+
+def test_masks_that_broadcast():
+    p = _policy()
+    B, Q, V = 3, 4, 343
+    x = _logits(B * Q, V, torch.float32).view(B, Q, V)
+    a = _actions(B * Q, V).view(B, Q)
+    g = torch.Generator().manual_seed(4)
+    for shape in ((V,), (1, V), (Q, V), (B, 1, V), (1, 1, V), (B, Q, V), (B, Q, 1)):
+        m = (torch.rand(shape, generator=g) < 0.5).cuda()
+        m[..., 0] = True
+        full = m.expand(B, Q, V).reshape(B * Q, V)
+        r = p.action_logprobs(x, a.cuda(), top=5, mask=m)
+        want = po.logprobs(x.view(-1, V), a, full, 1.0, 5)
+        po.check(r.entropy, *want["entropy"], "entropy")
+        assert torch.equal(r.top_ids.cpu().view(-1, 5), want["top_ids"].cpu())
+        t, ids = _teacher(x.view(-1, V), 6, full)
+        loss, tol, _, _ = po.distill(x.view(-1, V), t, ids, full, 1.0, True)
+        got = p.distill_loss(x, t.view(B, Q, 6).cuda(), ids.view(B, Q, 6).cuda(), mask=m, rest=True, reduction="none")
+        po.check(got, loss, tol, "loss")
+    y = _logits(2 * 3 * 4, 65, torch.bfloat16).view(2, 3, 4, 65)
+    z = y.transpose(0, 2)  # strides of three levels: copied
+    r = p.action_logprobs(z, top=3)
+    want = po.logprobs(z.reshape(-1, 65), None, None, 1.0, 3)
+    assert r.logp is None and r.entropy.shape == (4, 3, 2)
+    po.check(r.entropy, *want["entropy"], "entropy")
+    assert torch.equal(r.top_ids.cpu().view(-1, 3), want["top_ids"].cpu())
+
+
 def test_gradients_against_differences():
     """Central differences of the kernels' own f32 values, V = 9, step s = 2^-6: the third derivatives of these
     functions are under 4 (|logits| < 4, T = 1), so the difference is off by 4 s^2 / 6 < 2e-4, and by the values' own
@@ -421,7 +517,7 @@ def test_offsets_past_32_bits():
     x = row.expand(n, V)
     loss, d = p.distill_loss_grad(x, t.cuda().expand(n, 9), ids.cuda().expand(n, 9), rest=True, weight=1.0)
     lw, tol, dw, dd = po.distill(row, t, ids, None, 1.0, True)
-    one = torch.ones(1, 1, dtype=torch.float64)
+    one = torch.ones(1, 1, dtype=torch.float64, device="cuda")
     for r in (0, 16384, n - 1):
         po.check(d[r:r + 1], dw, po.grad_tol(dw, dd, one, torch.bfloat16), f"row {r}")
     po.check(loss, lw.sum() * n, tol.sum() * n + po.H * n * lw.sum().abs(), "total")
