@@ -187,6 +187,13 @@ __device__ __forceinline__ void apply_mask(const uint8_t* mk, float* f) {
     for (int i = 0; i < VN<T>; ++i) f[i] = b[i] ? f[i] : -INFINITY;
 }
 
+// 1 / x for x in the normal range: the instruction's estimate (2^-24 or better) and two Newton steps, which square its
+// error; a quarter of the division's instructions, correct to a few 2^-53
+__device__ __forceinline__ double rcp_f64(double x) {
+    double y = __builtin_amdgcn_rcp(x);
+    y = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
 // ln s in f64, s >= 0: s = 2^e f, f in [0.75, 1.5), ln f = 2 atanh(v), v = (f - 1) / (f + 1), |v| <= 0.2, by its power
 // series to v^15 (what is left is under 2e-13)
 __device__ __forceinline__ double ln_f64(double s) {
@@ -197,7 +204,7 @@ __device__ __forceinline__ double ln_f64(double s) {
         f *= 2.0;
         --e;
     }
-    const double v = (f - 1.0) / (f + 1.0), w = v * v;
+    const double v = (f - 1.0) * rcp_f64(f + 1.0), w = v * v;
     double t = 1.0 / 15;
     t = t * w + 1.0 / 13;
     t = t * w + 1.0 / 11;
@@ -1036,7 +1043,7 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
         if (id[u] >= 0) q[u] = exp_f64((double)e.t[u] - (double)h.tm);
     }
     h.qs = wave_sum(q[0] + q[1]);
-    const double iq = Te.rest || !h.any ? 1.0 : 1.0 / h.qs;
+    const double iq = Te.rest || !h.any ? 1.0 : rcp_f64(h.qs);  // qs >= 1: the largest entry is e^0
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int j = lane + 64 * u;
@@ -1498,13 +1505,24 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
         }
 }
 
-// out = scale sum_r w_r loss_r in a fixed order, f64
+// out = scale sum_r w_r loss_r in a fixed order, f64: one block, eight loads a thread in flight
 __global__ __launch_bounds__(1024) void loss_total_kernel(const float* __restrict__ loss, const float* w,
                                                           long long w_s, float scale, long long n,
                                                           float* __restrict__ out) {
     __shared__ double sh[16];
     double a = 0.0;
-    for (long long i = threadIdx.x; i < n; i += 1024) a += (double)loss[i] * (w ? (double)w[i * w_s] : 1.0);
+    long long i = threadIdx.x;
+    for (; i + 7 * 1024 < n; i += 8 * 1024) {
+        float l[8], g[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            l[u] = loss[i + u * 1024];
+            g[u] = w ? w[(i + u * 1024) * w_s] : 1.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) a += (double)l[u] * (double)g[u];
+    }
+    for (; i < n; i += 1024) a += (double)loss[i] * (w ? (double)w[i * w_s] : 1.0);
     a = wave_sum(a);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
     __syncthreads();
@@ -1519,7 +1537,8 @@ __global__ __launch_bounds__(1024) void loss_total_kernel(const float* __restric
 bool rows_of(const azg_logits* L, Rows* R) {
     if (!L || !L->x || L->rows < 1 || L->vocab < 1 || L->vocab > AZG_POLICY_VOCAB_MAX ||
         L->rows > AZG_POLICY_ROWS_MAX) return false;
-    if (L->inner < 1 || L->dtype < AZG_F32 || L->dtype > AZG_F16) return false;
+    if (L->inner < 1 || L->dtype < AZG_F32 || L->dtype > AZG_F16 || L->rows > (1LL << 60) / L->vocab) return false;
+    if (L->stride_outer < 0 || L->stride_inner < 0 || L->mask_outer < 0 || L->mask_inner < 0) return false;
     if (!(L->temperature > 0.f) || !std::isfinite(L->temperature)) return false;
     const double c = 1.4426950408889634074 / (double)L->temperature;
     *R = Rows{L->x, L->mask, L->rows, L->inner, L->stride_outer, L->stride_inner, L->mask_outer, L->mask_inner,

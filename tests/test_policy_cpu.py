@@ -87,7 +87,8 @@ def test_c_entries_refuse():
     p = f.data_ptr()
     bad = [dict(x=0), dict(rows=0), dict(rows=2 ** 40), dict(inner=0), dict(vocab=0), dict(vocab=2 ** 31),
            dict(dtype=3), dict(dtype=-1), dict(temperature=0.0), dict(temperature=math.nan), dict(temperature=math.inf),
-           dict(temperature=-1.0)]
+           dict(temperature=-1.0), dict(stride_inner=-5), dict(stride_outer=-1), dict(mask_inner=-1),
+           dict(rows=2 ** 34, vocab=2 ** 28)]
     t = policy._TEACHER(p, p, 0, 1, 3, 0)
     for kw in bad:
         g = logits(**kw)
