@@ -9,9 +9,10 @@ import math
 import torch
 
 H = 2.0 ** -24
-# the exponential's instruction returns 0 for results under the smallest normal number: a probability below 2^-126 may
-# be 0, which moves a gradient by at most 2^-126 times its factor (no sum of 2^30 such terms reaches h times a sum >= 1)
-FLUSHED = 2.0 ** -126
+# the exponential's instruction returns 0 for results under the smallest normal number, 2^-126, and what it is given is
+# 2^u = p s with s >= 2^-0.5 (the reference is the maximum's, rounded to a whole number): a probability below 2^-125.5 may
+# be 0, which moves a gradient by at most that times its factor (no sum of 2^30 such terms reaches h times a sum >= 1)
+FLUSHED = 2.0 ** -125.5
 TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
 
 
@@ -137,12 +138,15 @@ def distill(x, t_logp, t_ids, mask, T, rest):
         loss = loss + qr * (lqr - lr)
         lr = torch.where(may, lpr, torch.zeros_like(lpr))
         lqm = torch.maximum(qr, dS).clamp_min(1e-300).log()
-        tol = tol + torch.where(may, dS * ((lqr - lr).abs() + (lqm - lr).abs() + 1) + qr * (2 * sl + 4 * H * lr.abs()),
+        tol = tol + torch.where(may, dS * ((lqr - lr).abs() + (lqm - lr).abs() + 1) + qr * (2 * sl + 8 * H * lr.abs()),
                                 dS * 0)
         S = S + qr
-        pr = lr.exp()
-        rp = torch.where(out & has[:, None], p * (qr / pr)[:, None], torch.zeros_like(p))
-        dr = torch.where(out & may[:, None], p * (dS / pr)[:, None], torch.zeros_like(p)) + rp * 3 * sl[:, None]
+        # p / p_R from the logarithms: both may be 0 in f64
+        po = torch.where(out & may[:, None], (logp - lr[:, None]).exp(), torch.zeros_like(p))
+        rp = torch.where(has[:, None], po * qr[:, None], torch.zeros_like(p))
+        lpo = torch.where(po > 0, logp - lr[:, None], torch.zeros_like(p)).abs()
+        # p' has its own sum (its mean |u| beside that of sl) and its own logarithm
+        dr = po * dS[:, None] + rp * (3 * sl[:, None] + 8 * H * (lpo + 2) + 12 * H * (po * lpo).sum(1, keepdim=True))
     nothing = (lse == -math.inf) | ~there.any(1)
     loss = torch.where(nothing, torch.zeros_like(loss), loss)
     tol = tol + H * loss.abs().nan_to_num(0, 0, 0)
@@ -150,8 +154,7 @@ def distill(x, t_logp, t_ids, mask, T, rest):
         tgt = torch.where(mask.to(x.device).bool(), tgt, torch.zeros_like(tgt))
     d = torch.where(nothing[:, None], torch.zeros_like(p), (p * S[:, None] - tgt - rp) / T)
     lpa = torch.where(p > 0, logp, torch.zeros_like(p)).abs()
-    dd = p * S[:, None] * (3 * sl[:, None] + 8 * H * (lpa + 2)) + p * dS[:, None] + 16 * H * tgt + dr + \
-        rp * 8 * H * (lpa + 2) + FLUSHED * (1 + S[:, None])
+    dd = p * S[:, None] * (3 * sl[:, None] + 8 * H * (lpa + 2)) + p * dS[:, None] + 16 * H * tgt + dr + FLUSHED * (1 + S[:, None])
     return loss, tol, d, dd / T
 
 
@@ -162,8 +165,10 @@ def grad_tol(d, dd, w, dtype):
 
 
 def check(got, want, tol, what):
+    most = torch.finfo(got.dtype).max
     got = got.detach().double().reshape(want.shape)
     same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    same |= torch.isinf(got) & (got * want > 0) & (want.abs() > most)  # beyond the type's largest number
     off = torch.where(same, torch.zeros_like(want), (got - want).abs())
     bad = ~(same | (off <= tol))
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} off, first at "

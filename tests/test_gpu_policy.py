@@ -434,6 +434,66 @@ def test_masks_that_broadcast():
     assert torch.equal(r.top_ids.cpu().view(-1, 3), want["top_ids"].cpu())
 
 
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 0.1, 7.0, 1e3, 1e6])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_temperatures(T, dtype):
+    for n, V in ((5, 343), (3, 20011)):
+        x = _logits(n, V, DT[dtype])
+        _check_logprobs(x, _mask("random", n, V), _actions(n, V), 11, T=T)
+        t, ids = _teacher(x, 11, None)
+        for rest in (False, True):
+            _check_distill(x, None, t, ids, rest, T=T)
+
+
+def test_weights():
+    p = _policy()
+    x = _logits(12, 343, torch.float32)
+    t, ids = _teacher(x, 9, None)
+    t, ids = t.cuda(), ids.cuda()
+    loss, tol, d, dd = po.distill(x, t, ids, None, 1.0, True)
+    for w in (None, 2.0, 0.0, -1, torch.tensor(0.25), torch.tensor(0.25, dtype=torch.float64),
+              torch.arange(12).float() - 3, (torch.arange(12) * 0.5).bfloat16(), torch.arange(24).float()[::2],
+              torch.tensor(1.5).expand(12)):
+        wt = w.cuda() if isinstance(w, torch.Tensor) else w
+        got, g = p.distill_loss_grad(x, t, ids, rest=True, weight=wt)
+        full = torch.full((12,), 1 / 12 if w is None else float(w), dtype=torch.float64, device="cuda") \
+            if not isinstance(w, torch.Tensor) or w.dim() == 0 else wt.double()
+        total = (loss * full).sum()
+        po.check(got, total, (tol * full.abs()).sum() + po.H * (3 * loss * full.abs()).sum() + 1e-30, "total")
+        po.check(g, d * full[:, None], po.grad_tol(d, dd, full[:, None], x.dtype), "gradient")
+
+
+def test_strided_small_inputs():
+    """Actions, teacher entries and incoming gradients of other strides and types."""
+    p = _policy()
+    n, V, k = 10, 343, 7
+    x = _logits(n, V, torch.bfloat16)
+    a = _actions(n, V)
+    wide = torch.stack([a, a + 1], 1).cuda()
+    want = po.logprobs(x, a, None, 1.0, 0)
+    for act in (wide[:, 0], wide[:, 0].int(), torch.stack([a, a]).cuda()[1]):
+        po.check(p.action_logprobs(x, act).logp, *want["logp"], "logp")
+    t, ids = _teacher(x, k, None)
+    tt, ii = t.t().contiguous().cuda().t(), ids.t().contiguous().cuda().t()
+    loss, tol, d, dd = po.distill(x, t, ids, None, 1.0, False)
+    po.check(p.distill_loss(x, tt, ii, reduction="none"), loss, tol, "loss")
+    leaf = x.detach().requires_grad_(True)
+    g = torch.randn((n, 2), generator=torch.Generator().manual_seed(1)).cuda()
+    got, = torch.autograd.grad(p.distill_loss(leaf, tt, ii, reduction="none"), leaf, g[:, 1])
+    w = g[:, 1].double()[:, None]
+    po.check(got, d * w, po.grad_tol(d, dd, w, x.dtype), "gradient")
+    s = p.distill_loss(leaf, tt, ii, reduction="sum")
+    po.check(s, loss.sum(), tol.sum() + po.H * 2 * loss.sum().abs(), "sum")
+    got, = torch.autograd.grad(s, leaf)
+    one = torch.ones((1, 1), dtype=torch.float64, device="cuda")
+    po.check(got, d, po.grad_tol(d, dd, one, x.dtype), "gradient of the sum")
+    # only one of the outputs used
+    q = p.action_logprobs(leaf, wide[:, 0])
+    got, = torch.autograd.grad(q.lse, leaf, g[:, 0])
+    dw, tw = po.logprobs_grad(x, a, None, 1.0, None, None, g[:, 0])
+    po.check(got, dw, tw, "gradient of lse")
+
+
 def test_gradients_against_differences():
     """Central differences of the kernels' own f32 values, V = 9, step s = 2^-6: the third derivatives of these
     functions are under 4 (|logits| < 4, T = 1), so the difference is off by 4 s^2 / 6 < 2e-4, and by the values' own
