@@ -125,9 +125,13 @@ constexpr int block_of = TEAM == 64 ? 256 : TEAM;
 template <int TEAM>
 __device__ __forceinline__ int team_tid() { return TEAM == 64 ? threadIdx.x & 63 : threadIdx.x; }
 template <int TEAM>
-__device__ __forceinline__ int team_in_block() { return TEAM == 64 ? threadIdx.x >> 6 : 0; }
+__device__ __forceinline__ int team_in_block() {  // by readfirstlane: the same for a wave, so its row is scalar work
+    return TEAM == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+}
 template <int TEAM>
-__device__ __forceinline__ long long team_row() { return TEAM == 64 ? block_row() * 4 + (threadIdx.x >> 6) : block_row(); }
+__device__ __forceinline__ long long team_row() {
+    return TEAM == 64 ? block_row() * 4 + team_in_block<TEAM>() : block_row();
+}
 
 // ---- vectors of 16 bytes ------------------------------------------------------------------------------
 // A row may start at any element and so may its vectors (the loads need no more than the element's alignment; vectors
@@ -670,9 +674,10 @@ __device__ int top_select(const T* x, const uint8_t* mk, int V, int k, bool plai
         team_sync<TEAM>();
         const int nh = S.nh;
         if (nh <= S.HITS) {
-            const int per = nvec >= TEAM * GROUP ? GROUP : nvec > TEAM ? (nvec + TEAM - 1) / TEAM : 1;  // vectors a group has
-            for (int i = tid; i < nh * per; i += TEAM) {
-                const int h = S.hits[i / per], u = i % per, g = h / TEAM, t = h % TEAM;
+            const int sh = nvec > 2 * TEAM ? 2 : nvec > TEAM ? 1 : 0;  // 2^sh vectors a group has
+            static_assert(GROUP == 4, "sh");
+            for (int i = tid; i < nh << sh; i += TEAM) {
+                const int h = S.hits[i >> sh], u = i & ((1 << sh) - 1), g = h / TEAM, t = h % TEAM;
                 float f[N];
                 int i0, n = 0;
                 if (g == ng) {
@@ -693,7 +698,10 @@ __device__ int top_select(const T* x, const uint8_t* mk, int V, int k, bool plai
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     if (j >= n || !(f[j] >= bv)) continue;
-                    const unsigned long long key = order_key(f[j], i0 + j);
+                    const int b = (int)__float_as_uint(f[j] + 0.f);  // order_key without its NaN
+                    const unsigned long long key =
+                        ((unsigned long long)((unsigned)b ^ (unsigned)((b >> 31) | 0x80000000)) << 32) |
+                        (0xFFFFFFFFu - (unsigned)(i0 + j));
                     if (key < bound) continue;
                     const int at = atomicAdd(&S.nc, 1);
                     if (at < S.CANDS) S.cand[at] = key;
