@@ -881,6 +881,19 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
     }
 }
 
+// A gradient kernel's row, or its part of one: rows from the last to the first, a row's parts next to each other
+// (across rows first, the blocks at work touch memory all over: 354 us against 300, 2048 x 100003 f32).
+struct Part {
+    long long r;
+    int from;
+};
+template <int TEAM>
+__device__ __forceinline__ Part part_of(const Rows& R, int len) {
+    const unsigned n = ((unsigned)R.V + (unsigned)len - 1) / (unsigned)len;
+    const long long id = team_row<TEAM>(), q = n == 1 ? id : id / n;
+    return Part{R.rows - 1 - q, (int)(id - q * n) * len};
+}
+
 // Elementwise over a row or a part of it: f(x, legal) for each element, vectors of 16 bytes.  Rows are taken from
 // the last to the first: what a forward pass read last may still be in the Infinity Cache.
 template <class T, int TEAM, bool MASK, bool NT, class F>
@@ -939,9 +952,10 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, co
                                                            long long gl_s, const float* ge, long long ge_s,
                                                            const float* gz, long long gz_s, T* __restrict__ dx,
                                                            int len, bool nt) {
-    const long long r = R.rows - 1 - team_row<TEAM>();
+    const Part at = part_of<TEAM>(R, len);
+    const long long r = at.r;
     if (r < 0) return;
-    const int from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
+    const int from = at.from, V = R.V - from < len ? R.V - from : len;
     const T* x = row_ptr<T>(R, r) + from;
     const uint8_t* mk = MASK ? mask_ptr(R, r) + from : nullptr;
     const float4 st = ((const float4*)stats)[r];
@@ -954,19 +968,19 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, co
     const float c1 = g2 * R.invT * LN2 / s, ga = g1 * R.invT;
     const float c0 = (g3 - g1 - g2 * H) * R.invT / s + c1 * lg2(s);
     T* d = dx + r * (long long)R.V + from;
-    const int at = given ? (int)(a - from) : -1;  // outside this part: no element's index
+    const int mine = given ? (int)(a - from) : -1;  // outside this part: no element's index
     if (s == 0.f) {  // no legal action
         map_row<T, TEAM, false>(x, mk, d, V, nt, [](float, int) { return 0.f; });
     } else if (st.w != 0.f) {
         map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int i) {
             const float u = nmax((y - ref) * R.c, -1000.f);
-            return ex2(u) * (c0 - c1 * u) + (i == at ? ga : 0.f);
+            return ex2(u) * (c0 - c1 * u) + (i == mine ? ga : 0.f);
         });
     } else {
         map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int i) {
             const float u = nmax(__builtin_fmaf(y, R.c, -ref), -1000.f);
             const float g = ex2(u) * __builtin_fmaf(-c1, u, c0);
-            return i == at ? g + ga : g;
+            return i == mine ? g + ga : g;
         });
     }
 }
@@ -997,10 +1011,10 @@ struct EntryRegs {  // as loaded, an entry or two a lane
     bool legal[2];
 };
 
-// by one wave; nothing here waits for the last loads: what a team loads of the row comes behind them
+// by one wave, with the logits of the entries in [lo, hi); nothing here waits for the last loads: what a team loads of the row comes behind them
 template <class T>
-__device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long r, int V, const T* x,
-                                                   const uint8_t* mk) {
+__device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long r, int V, const T* x, const uint8_t* mk,
+                                                   int lo, int hi) {
     const int lane = threadIdx.x & 63;
     EntryRegs e;
 #pragma unroll
@@ -1022,7 +1036,8 @@ __device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (64 * u >= Te.k) continue;
-        const int i = e.id[u] < 0 ? 0 : e.id[u];
+        const int i = e.id[u];
+        if (i < lo || i >= hi) continue;  // -1 as well
         e.x[u] = (float)x[i];
         e.legal[u] = !mk || mk[i];
     }
@@ -1265,7 +1280,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     Entries& E = Es[mine];
     // the entries' loads first: they are few, and the row's come behind them
     EntryRegs er;
-    if (tid < 64) er = fetch_entries<T>(Te, r, V, x, mk);
+    if (tid < 64) er = fetch_entries<T>(Te, r, V, x, mk, 0, V);
     constexpr int U = NV * N >= 16 ? 16 / N : 1, Q = NV > 0 ? NV / U : 1;  // 16 logits unpacked at a time
     Loaded<T, U> L[Q];
     if constexpr (NV > 0) {
@@ -1442,9 +1457,11 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     __shared__ Entries Es[TEAMS];
     __shared__ Row row;
     __shared__ Stat<false> joined;
-    const long long r = R.rows - 1 - team_row<TEAM>();
+    // from parts: few rows, or long ones whose many coefficients a block should not work out for little of it
+    const Part at = JOIN ? Part{R.rows - 1 - team_row<TEAM>(), (int)blockIdx.z * len} : part_of<TEAM>(R, len);
+    const long long r = at.r;
     if (r < 0) return;
-    const int tid = team_tid<TEAM>(), from = blockIdx.z * len, V = R.V - from < len ? R.V - from : len;
+    const int tid = team_tid<TEAM>(), from = at.from, V = R.V - from < len ? R.V - from : len;
     const T* x = row_ptr<T>(R, r);
     const uint8_t* mk = MASK ? mask_ptr(R, r) : nullptr;
     Entries& E = Es[team_in_block<TEAM>()];
@@ -1454,7 +1471,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     if constexpr (JOIN)
         if (tid < P.n) part = P.part[r * P.n + tid];
     if (tid < 64) {
-        h = load_entries<T>(E, fetch_entries<T>(Te, r, R.V, x, mk), Te, R.c);
+        h = load_entries<T>(E, fetch_entries<T>(Te, r, R.V, x, mk, JOIN ? 0 : from, JOIN ? R.V : from + V), Te, R.c);
         if constexpr (JOIN) repeats = find_repeats(E, Te.k);
     }
     Row o;
@@ -1644,7 +1661,9 @@ unsigned bits_bytes(int V) {
 }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
-constexpr int BWD_LEN = 16384;  // elements of a row that a block of a gradient kernel takes
+// a block of a gradient kernel takes 16 KB of a row, four vectors a thread and no loop
+template <class T>
+constexpr int bwd_len = 16384 / (int)sizeof(T);
 
 template <class T, bool MASK>
 void distill_bwd(const Rows& R, const Teacher& Te, const DistillOut& O, hipStream_t st) {
@@ -1654,8 +1673,8 @@ void distill_bwd(const Rows& R, const Teacher& Te, const DistillOut& O, hipStrea
                            none, R.V);
     else
         hipLaunchKernelGGL((distill_bwd_kernel<T, 256, MASK, false>),
-                           team_grid<256>(R.rows, (R.V + BWD_LEN - 1) / BWD_LEN), dim3(256), 0, st, R, Te, O, none,
-                           BWD_LEN);
+                           team_grid<256>(R.rows * ((R.V + bwd_len<T> - 1) / bwd_len<T>)), dim3(256), 0, st, R, Te, O, none,
+                           bwd_len<T>);
 }
 
 template <class T, int TEAM, bool MASK, int NV>
@@ -1772,10 +1791,10 @@ extern "C" int azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_
                                    too_large<T>(R));
             else
                 hipLaunchKernelGGL((logprobs_bwd_kernel<T, 256, MASK>),
-                                   team_grid<256>(R.rows, (R.V + BWD_LEN - 1) / BWD_LEN), dim3(256), 0,
+                                   team_grid<256>(R.rows * ((R.V + bwd_len<T> - 1) / bwd_len<T>)), dim3(256), 0,
                                    (hipStream_t)stream, R, actions, actions64, stats, g_logp, (long long)g_logp_stride,
                                    g_entropy, (long long)g_entropy_stride, g_lse, (long long)g_lse_stride, (T*)dx,
-                                   BWD_LEN, too_large<T>(R));
+                                   bwd_len<T>, too_large<T>(R));
             return 0;
         });
     });
