@@ -1260,8 +1260,15 @@ __device__ __forceinline__ float row_weight(const Rows& R, const DistillOut& O, 
 
 // A team a row: statistics, loss and (dx) the gradient.  NV > 0: the row stays in registers (NV vectors a thread)
 // between its two uses, and HBM sees it once; NV = 0: it is read again from the cache.
+// Waves that a SIMD has to hold (the compiler keeps to the registers that leaves): all eight for a wave's short rows (86 us
+// against 97 with the 5 it took by itself, step 65536 x 343 f32); 6 for up to 8 vectors a thread (203 us with 512 threads
+// against 230 with 256 threads of 16 vectors and 4 waves, step 8192 x 32768 bf16: three rows of 64 KB a CU either
+// way, and half the serial work); 4 for 16 vectors.
+template <int TEAM, int NV>
+constexpr int waves_of = NV > 8 ? 4 : TEAM == 64 && NV <= 2 ? 8 : 6;
+
 template <class T, int TEAM, bool MASK, int NV>
-__global__ __launch_bounds__(block_of<TEAM>) __attribute__((amdgpu_waves_per_eu(4)))  // four rows of 64 KB a CU
+__global__ __launch_bounds__(block_of<TEAM>) __attribute__((amdgpu_waves_per_eu(waves_of<TEAM, NV>)))
 void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     extern __shared__ unsigned bits_all[];
     constexpr int TEAMS = block_of<TEAM> / TEAM, N = VN<T>;
@@ -1704,8 +1711,8 @@ void distill_fwd(const Rows& R, const Teacher& Te, const DistillOut& O, Split P,
         distill_rows<T, 64, MASK, 8>(R, Te, O, st);
     } else if (V <= 256 * N * 8) {
         distill_rows<T, 256, MASK, 8>(R, Te, O, st);
-    } else if (V <= 256 * N * 16) {
-        distill_rows<T, 256, MASK, 16>(R, Te, O, st);
+    } else if (V <= 512 * N * 8) {
+        distill_rows<T, 512, MASK, 8>(R, Te, O, st);
     } else if (V <= 512 * N * 16) {
         distill_rows<T, 512, MASK, 16>(R, Te, O, st);
     } else {
