@@ -11,8 +11,17 @@
 //       (S = sum q_j + q_R, p' = p / p_R by the outside's own maximum and sum: p_R may be far below the
 //       smallest f32 where the entries hold nearly everything)
 //
-// Sums are over the legal actions (a byte mask, or all).  Logits are f32, bf16 or f16; statistics are f32, the
-// few terms of a row's KL (a difference of near values) f64.
+// Sums are over the legal actions (a byte mask, or all).  Logits are f32, bf16 or f16; a row's statistics are f32,
+// those of a KL (a difference of near values) and its few terms f64.
+//
+// All of it is bound by HBM from some thousand rows x columns on, by chains of dependent steps and the call below.
+// On an MI355X (a 1 GiB copy reaches 5.2 TB/s, reading alone 6.4):
+//   scores, 8192 x 32768 bf16, top 8             93 us   5.8 TB/s of reads
+//   scores and gradient, 4092 x 50001 bf16       76 + 132 us (the second from the caches in part)
+//   loss alone, 4096 x 65536 f16, 16 entries     86 us   6.3 TB/s of reads
+//   loss with gradient, 8192 x 32768 bf16, 32   202 us   5.3 TB/s read and written once
+//   loss, then gradient, 2048 x 100003 f32, 128 138 + 300 us, 5.5 TB/s over both
+//   1 x 131072 bf16, top 20                      6.9 + 5.5 us (32 parts, joined)
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -108,7 +117,9 @@ __device__ __forceinline__ V wave_reduce(V x, F f) {
 }
 template <class V>
 __device__ __forceinline__ V wave_sum(V x) { return wave_reduce(x, [](V a, V b) { return a + b; }); }
-__device__ __forceinline__ float wave_max(float x) { return wave_reduce(x, [](float a, float b) { return nmax(a, b); }); }
+__device__ __forceinline__ float wave_max(float x) {
+    return wave_reduce(x, [](float a, float b) { return nmax(a, b); });
+}
 
 // A team is the threads that share a row: a wave (64; four teams in a block) or a block.
 template <int TEAM>
@@ -409,8 +420,8 @@ struct NoEdit {
 };
 
 template <class T, int TEAM, bool MASK, bool ENT, bool TOP, bool NT, class Edit>
-__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum<ENT>& a, float& mx, Best& best,
-                                         float* gmax, const Edit& edit) {
+__device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, float c, Sum<ENT>& a, float& mx,
+                                         Best& best, float* gmax, const Edit& edit) {
     constexpr int N = VN<T>;
     const int tid = team_tid<TEAM>(), nvec = V / N, step = TEAM * GROUP;
     // a vector's elements and maximum
@@ -579,7 +590,8 @@ __device__ __forceinline__ int rank_in(const unsigned long long* arr, unsigned l
 
 // a bound of the k-th largest of a row from its threads' best.  A wave by ballots (75 us against 82 with ranks, 65536 x
 // 343 f32, top 16: the fewest instructions).  A block by ranks in LDS, each wave for itself over 64 groups of
-// threads where these are enough (the shorter chain: 91 us against 98, 8192 x 32768 bf16, top 8), else over all.
+// threads where these are enough (the shorter chain: 91 us against 98, 8192 x 32768 bf16, top 8), else over 128 pairs
+// (35 us against 39 over all, 2000 x 32768 bf16, top 50) or over all.
 template <int TEAM>
 __device__ __forceinline__ unsigned long long kth_best(unsigned long long best, int k, TopShare<TEAM>& S) {
     const int tid = team_tid<TEAM>(), lane = threadIdx.x & 63;
@@ -601,10 +613,21 @@ __device__ __forceinline__ unsigned long long kth_best(unsigned long long best, 
             __syncthreads();  // arr becomes the candidates
             return at ? lane_of(me, __builtin_ctzll(at)) : 0;
         }
-        arr[tid] = best;
-        __syncthreads();
-        if (best != 0 && rank_in<TEAM>(arr, best) == k - 1) S.bound = best;
-        __syncthreads();
+        if (k <= 64) {  // 128 pairs of threads, by two waves
+            const unsigned long long b = dpp<QUAD_XOR1>(best);
+            best = best > b ? best : b;
+            if ((tid & 1) == 0) arr[tid / 2] = best;
+            __syncthreads();
+            if (tid < 128) {
+                const unsigned long long me = arr[tid];
+                if (me != 0 && rank_in<128>(arr, me) == k - 1) S.bound = me;
+            }
+        } else {
+            arr[tid] = best;
+            __syncthreads();
+            if (best != 0 && rank_in<TEAM>(arr, best) == k - 1) S.bound = best;
+        }
+        __syncthreads();  // and arr becomes the candidates
         return S.bound;
     }
 }
@@ -745,8 +768,8 @@ __device__ __forceinline__ long long action_of(const LogprobsOut& O, long long r
 }
 
 template <class T>
-__device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat<true>& st, float l2,
-                                          long long act, const T* x, const uint8_t* mk) {
+__device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat<true>& st,
+                                          float l2, long long act, const T* x, const uint8_t* mk) {
     const bool empty = st.s == 0.f;
     const float H = empty ? 0.f : LN2 * (l2 - st.w / st.s);
     if (O.stats) ((float4*)O.stats)[r] = make_float4(st.ref, st.s, H, st.wide ? 1.f : 0.f);
@@ -1011,7 +1034,8 @@ struct EntryRegs {  // as loaded, an entry or two a lane
     bool legal[2];
 };
 
-// by one wave, with the logits of the entries in [lo, hi); nothing here waits for the last loads: what a team loads of the row comes behind them
+// by one wave, with the logits of the entries in [lo, hi) alone; nothing here waits for the last loads, so that what a
+// team loads of the row comes right behind them
 template <class T>
 __device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long r, int V, const T* x, const uint8_t* mk,
                                                    int lo, int hi) {
@@ -1260,10 +1284,10 @@ __device__ __forceinline__ float row_weight(const Rows& R, const DistillOut& O, 
 
 // A team a row: statistics, loss and (dx) the gradient.  NV > 0: the row stays in registers (NV vectors a thread)
 // between its two uses, and HBM sees it once; NV = 0: it is read again from the cache.
-// Waves that a SIMD has to hold (the compiler keeps to the registers that leaves): all eight for a wave's short rows (86 us
-// against 97 with the 5 it took by itself, step 65536 x 343 f32); 6 for up to 8 vectors a thread (203 us with 512 threads
-// against 230 with 256 threads of 16 vectors and 4 waves, step 8192 x 32768 bf16: three rows of 64 KB a CU either
-// way, and half the serial work); 4 for 16 vectors.
+// Waves that a SIMD has to hold (the compiler keeps to the registers that leaves): all eight for a wave's short rows
+// (86 us against 97 with the 5 it took by itself, step 65536 x 343 f32); 6 for up to 8 vectors a thread (203 us
+// with 512 threads against 230 with 256 threads of 16 vectors and 4 waves, step 8192 x 32768 bf16: three rows of
+// 64 KB a CU against four, each with half the serial work); 4 for 16 vectors.
 template <int TEAM, int NV>
 constexpr int waves_of = NV > 8 ? 4 : TEAM == 64 && NV <= 2 ? 8 : 6;
 
@@ -1354,7 +1378,8 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         Best none{-INFINITY, 0};
         row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
-    const Stat<false> v = row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
+    const Stat<false> v =
+        row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
     if (tid < 64) {
         RowSums both;
         const Row o = row_coefficients(R, Te, E, h, v, repeats, &both);
@@ -1444,7 +1469,8 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
     Sum<false> a{-FAR, 0.0, 0.f};
     float mx = -INFINITY;
     Best none{-INFINITY, 0};
-    row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, SkipBits<T>{bits, Te.rest != 0}, r < O.keep);
+    const SkipBits<T> skip{bits, Te.rest != 0};
+    row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     a = team_sum<256, false>(a, sh.sum);
     const bool plain = plain_sum(a);
     const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
@@ -1458,7 +1484,8 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
 // a row or a part of it of the gradient, from the row's statistics (stats) or from its parts (JOIN: then the first
 // part's block writes the row's loss and statistics as well)
 template <class T, int TEAM, bool MASK, bool JOIN>
-__global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Teacher Te, DistillOut O, Split P, int len) {
+__global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Teacher Te, DistillOut O, Split P,
+                                                                     int len) {
     constexpr int TEAMS = block_of<TEAM> / TEAM;
     __shared__ Shared<false> sh;
     __shared__ Entries Es[TEAMS];
@@ -1582,6 +1609,7 @@ int launched() {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : azg_host_fail(AZG_ERR_HIP, std::string("azg_policy: ") + hipGetErrorString(e));
 }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int bad(const char* what) { return azg_host_fail(AZG_ERR_ARG, what); }
 
 template <class F>
@@ -1616,9 +1644,11 @@ long long keep_from(const Rows& R, bool backward) {
 template <class T>
 bool too_large(const Rows& R) { return R.rows * R.V * (int)sizeof(T) > CACHE_BYTES / 2; }
 
-// Which team takes a row.  A wave: rows of up to 4 KB (a block would leave most of its threads idle).  A block:
-// longer ones.  Parts: rows longer than a block holds the maxima or bits (LDS) or the logits (registers) of, and, where there are fewer rows
-// than would fill the chip, rows of more than 8192 elements, in parts of 4096 or more.
+// Which team takes a row.  A wave: rows of up to 4 KB, and of up to 16 KB where there are waves enough (94 us against
+// 242, 38364 x 1135 f32, top 35; 58 against 89, 20000 x 4096 bf16: a block leaves most of its threads idle and pays for
+// its reductions).  A block: longer ones.  Parts: rows longer than a block holds the maxima or bits (LDS) or the logits
+// (registers) of; and rows of more than 8192 elements where there are fewer than 128, in parts of 4096 or more (with
+// 128 to 1024 rows parts were slower: 58 us against 44, 802 x 89386 f16, top 87).
 constexpr int WAVE_BYTES = 4096, WAVE_ROWS = 2048, PART_MIN = 4096;
 template <class T>
 int logprobs_most(bool top) { return top ? 1024 * 16 * VN<T> : 1 << 30; }
@@ -1761,7 +1791,7 @@ extern "C" int azg_logprobs_fwd(const azg_logits* L, const void* actions, int32_
                                 int64_t work_bytes, void* stream) {
     Rows R;
     if (!rows_of(L, &R) || !entropy || !lse || (actions != nullptr) != (logp != nullptr) || top < 0 || top > TOP_MAX ||
-        (top > 0 && (!top_logp || !top_ids)))
+        (top > 0 && (!top_logp || !top_ids)) || !aligned16(stats) || !aligned16(work))
         return bad("azg_logprobs_fwd: bad argument");
     const int64_t need = azg_logprobs_work(L, top);
     if (need > 0 && (!work || work_bytes < need)) return bad("azg_logprobs_fwd: work is too small");
@@ -1786,7 +1816,8 @@ extern "C" int azg_logprobs_bwd(const azg_logits* L, const void* actions, int32_
                                 int64_t g_entropy_stride, const float* g_lse, int64_t g_lse_stride, void* dx,
                                 void* stream) {
     Rows R;
-    if (!rows_of(L, &R) || !stats || !dx || (g_logp && !actions)) return bad("azg_logprobs_bwd: bad argument");
+    if (!rows_of(L, &R) || !stats || !dx || (g_logp && !actions) || !aligned16(stats))
+        return bad("azg_logprobs_bwd: bad argument");
     by_type(L->dtype, [&](auto z) {
         using T = decltype(z);
         return by_mask(R, [&](auto m) {
@@ -1813,7 +1844,8 @@ extern "C" int azg_distill_fwd(const azg_logits* L, const azg_teacher* t, float*
                                void* work, int64_t work_bytes, void* stream) {
     Rows R;
     Teacher Te;
-    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !row_loss) return bad("azg_distill_fwd: bad argument");
+    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !row_loss || !aligned16(stats) || !aligned16(work))
+        return bad("azg_distill_fwd: bad argument");
     const int64_t need = azg_distill_work(L, dx != nullptr);
     if (need > 0 && (!work || work_bytes < need)) return bad("azg_distill_fwd: work is too small");
     hipStream_t st = (hipStream_t)stream;
@@ -1837,7 +1869,7 @@ extern "C" int azg_distill_bwd(const azg_logits* L, const azg_teacher* t, const 
                                int64_t weight_stride, float scale, void* dx, void* stream) {
     Rows R;
     Teacher Te;
-    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !stats || !dx) return bad("azg_distill_bwd: bad argument");
+    if (!rows_of(L, &R) || !teacher_of(t, &Te) || !stats || !dx || !aligned16(stats)) return bad("azg_distill_bwd: bad argument");
     DistillOut O{const_cast<float*>(stats), nullptr, weight, (long long)weight_stride, scale, dx, 0, false};
     by_type(L->dtype, [&](auto z) {
         using T = decltype(z);

@@ -331,7 +331,8 @@ def distill_loss_grad(logits, teacher_logp, teacher_ids, *, temperature=1.0, mas
     """(loss, gradient) of sum_r weight_r KL_r (distill_loss's rows) in one call: what a training step needs, with
     one pass over the logits less than autograd.  weight: a number, or a tensor [...] of one per row; None: 1 / rows
     (the mean).  The loss is 0-dim f32, the gradient has the logits' shape and type (a new contiguous tensor):
-    logits.backward(gradient).  No autograd graph is built."""
+    logits.backward(gradient).  No autograd graph is built: in a training step captured in a HIP graph, or with the
+    loss scaled from outside (weight), this is the form to take."""
     t = _check_logits("distill_loss_grad", logits, temperature)
     mask = _check_mask("distill_loss_grad", logits, mask)
     t_logp, t_ids = _check_teacher("distill_loss_grad", logits, teacher_logp, teacher_ids)

@@ -119,3 +119,10 @@ def test_c_entries_refuse():
     assert L.azg_logprobs_fwd(g, None, 0, 0, None, None, p, p, None, None, None, 0, None) == -1
     assert L.azg_distill_fwd(g, t, p, p, None, 0, 1.0, None, p, p, 16, None) == -1
     assert b"work" in L.azg_last_error()
+    # statistics and scratch memory at 16 bytes
+    g = logits()
+    assert L.azg_logprobs_fwd(g, None, 0, 0, p + 4, None, p, p, None, None, None, 0, None) == -1
+    assert L.azg_logprobs_bwd(g, None, 0, p + 8, None, 0, p, 0, None, 0, p, None) == -1
+    assert L.azg_distill_fwd(g, t, p + 4, p, None, 0, 1.0, None, p, None, 0, None) == -1
+    assert L.azg_distill_fwd(g, t, p, p, None, 0, 1.0, None, p, p + 4, 2 ** 20, None) == -1
+    assert L.azg_distill_bwd(g, t, p + 4, None, 0, 1.0, p, None) == -1
