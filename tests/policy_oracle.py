@@ -141,10 +141,14 @@ def distill(x, t_logp, t_ids, mask, T, rest):
         tol = tol + torch.where(may, dS * ((lqr - lr).abs() + (lqm - lr).abs() + 1) + qr * (2 * sl + 8 * H * lr.abs()),
                                 dS * 0)
         S = S + qr
-        # p / p_R from the logarithms: both may be 0 in f64
-        po = torch.where(out & may[:, None], (logp - lr[:, None]).exp(), torch.zeros_like(p))
+        # p / p_R by the outside's own maximum: p and p_R may both be 0 in f64
+        zo = torch.where(out, z, torch.full_like(z, -math.inf))
+        zo = zo - torch.where(may[:, None], zo.max(1, keepdim=True).values, torch.zeros_like(lr)[:, None])
+        eo = torch.where(out & may[:, None], zo.exp(), torch.zeros_like(p))
+        so = eo.sum(1, keepdim=True).clamp_min(1e-300)
+        po = eo / so
         rp = torch.where(has[:, None], po * qr[:, None], torch.zeros_like(p))
-        lpo = torch.where(po > 0, logp - lr[:, None], torch.zeros_like(p)).abs()
+        lpo = torch.where(po > 0, zo - so.log(), torch.zeros_like(p)).abs()
         # p' has its own sum (its mean |u| beside that of sl) and its own logarithm
         dr = po * dS[:, None] + rp * (3 * sl[:, None] + 8 * H * (lpo + 2) + 12 * H * (po * lpo).sum(1, keepdim=True))
     nothing = (lse == -math.inf) | ~there.any(1)
