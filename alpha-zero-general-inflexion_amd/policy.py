@@ -169,7 +169,12 @@ def _logprobs(logits, actions, top, t, mask, want_stats):
     lead, dev = logits.shape[:-1], logits.device
     logits, mask, n, L = _rows(logits, mask, t)
     logp = top_logp = top_ids = stats = None
-    if actions is None:
+    if want_stats:  # tensors of their own: autograd lets nobody write into views that a Function returns
+        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        lse = torch.empty(lead, dtype=torch.float32, device=dev)
+        if actions is not None:
+            logp = torch.empty(lead, dtype=torch.float32, device=dev)
+    elif actions is None:
         entropy, lse = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind(0)
     else:
         entropy, lse, logp = torch.empty((3, *lead), dtype=torch.float32, device=dev).unbind(0)

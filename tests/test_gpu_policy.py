@@ -494,6 +494,36 @@ def test_strided_small_inputs():
     po.check(got, dw, tw, "gradient of lse")
 
 
+def test_results_may_be_written():
+    """The results are the caller's: changed in place, with and without a graph behind them."""
+    p = _policy()
+    x = _logits(6, 65, torch.float32)
+    a = _actions(6, 65)
+    keep = torch.tensor([1.0, 0.0, 1.0, 1.0, 0.0, 1.0])
+    leaf = x.clone().requires_grad_(True)
+    r = p.action_logprobs(leaf, a.cuda(), top=3)
+    r.logp.mul_(keep.cuda())
+    r.entropy.add_(1.0)
+    r.lse.zero_()
+    r.top_logp.exp_()
+    (r.logp.sum() + r.entropy.sum() + r.lse.sum()).backward()
+    dw, tol = po.logprobs_grad(x, a, None, 1.0, keep, torch.ones(6), None)
+    po.check(leaf.grad, dw, tol, "gradient")
+    with torch.no_grad():
+        q = p.action_logprobs(leaf, a.cuda())
+        want = po.logprobs(x, a, None, 1.0, 0)
+        q.logp.zero_()
+        po.check(q.entropy, *want["entropy"], "entropy")
+        po.check(q.lse, *want["lse"], "lse")
+    t, ids = _teacher(x, 5, None)
+    rows = p.distill_loss(leaf, t.cuda(), ids.cuda(), reduction="none")
+    rows.mul_(keep.cuda())
+    g, = torch.autograd.grad(rows.sum(), leaf)
+    _, _, d, dd = po.distill(x, t, ids, None, 1.0, False)
+    w = keep.double().cuda()[:, None]
+    po.check(g, d * w, po.grad_tol(d, dd, w, x.dtype), "weighted rows")
+
+
 def test_gradients_against_differences():
     """Central differences of the kernels' own f32 values, V = 9, step s = 2^-6: the third derivatives of these
     functions are under 4 (|logits| < 4, T = 1), so the difference is off by 4 s^2 / 6 < 2e-4, and by the values' own
