@@ -208,7 +208,7 @@ class _ActionLogprobs(torch.autograd.Function):
         logits, mask, actions, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:
             return None, None, None, None, None
-        _, _, n, L = _rows(logits, mask, ctx.t)
+        logits, mask, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if n:
             (a, sa), (e, se), (z, sz) = _spread(g_logp), _spread(g_entropy), _spread(g_lse)
@@ -295,7 +295,7 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, mask, t_logp, t_ids, stats = ctx.saved_tensors
-        _, _, n, L = _rows(logits, mask, ctx.t)
+        logits, mask, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if n:
             w, ws = _spread(g)
