@@ -230,9 +230,11 @@ __device__ __forceinline__ double ln_f64(double s) {
     t = t * w + 1.0;
     return 0.69314718055994530942 * e + 2.0 * v * t;
 }
-// e^t in f64: t = n ln 2 + z, |z| <= 0.35, its power series to z^9 (what is left is under 1e-11 of it)
+// e^t in f64: t = n ln 2 + z, |z| <= 0.35, its power series to z^9 (what is left is under 1e-11 of it).  0 below
+// -800 (f64 ends at -745): an entry at the type's lowest value would leave a z whose powers pass f64.  A NaN stays.
 __device__ __forceinline__ double exp_f64(double t) {
-    const double n = fmin(fmax(rint(t * 1.4426950408889634074), -2000.0), 2000.0);
+    t = t < -800.0 ? -800.0 : t;
+    const double n = fmin(rint(t * 1.4426950408889634074), 2000.0);
     const double z = __builtin_fma(n, -0.69314718055994530942, t);
     double p = 1.0 / 362880;
     p = p * z + 1.0 / 40320;
