@@ -370,6 +370,8 @@ struct Stat {
 __device__ __forceinline__ float u_of(float x, float ref, bool wide, float c) {
     return wide ? (x - ref) * c : __builtin_fmaf(x, c, -ref);
 }
+// the reference in units of x c (48 bits of a product: exact)
+__device__ __forceinline__ double place(float ref, bool wide, float c) { return wide ? (double)ref * (double)c : ref; }
 // the log-probability of a logit, l2 = log2 of the row's sum
 __device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2, float c, float invT) {
     if (st.wide) return (x - st.ref) * invT - LN2 * l2;
@@ -527,12 +529,10 @@ union Shared {  // one reduction at a time
 // a row's statistics from its pass: as they are, or by the element-wise pass; an empty row has s = 0
 template <class T, int TEAM, bool ENT, class Skip>
 __device__ __forceinline__ Stat<ENT> row_stat(Sum<ENT> a, float mx, const T* x, const uint8_t* mk, int V, float c,
-                                              Shared<ENT>& sh, bool again, Skip skip) {
+                                              Shared<ENT>& sh, Skip skip) {
     a = team_sum<TEAM, ENT>(a, sh.sum);
-    if (!again) {
-        if (plain_sum(a)) return Stat<ENT>{a.r, a.s, a.w, false};
-        if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat<ENT>{0.f, 0, 0.f, false};
-    }
+    if (plain_sum(a)) return Stat<ENT>{a.r, a.s, a.w, false};
+    if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat<ENT>{0.f, 0, 0.f, false};
     const Soft v = soft_pass<T, TEAM>(x, mk, V, c, sh.soft, skip);
     return Stat<ENT>{v.m, v.s, v.w, true};
 }
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
         st.wide = !plain && all != -INFINITY;
         if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, plain ? a.w : 0.f, st.wide);
     } else {
-        st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, false, [](int) { return false; });
+        st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, [](int) { return false; });
         l2 = lg2(st.s);
         if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
     }
@@ -1028,7 +1028,7 @@ struct Entries {
 struct EntryHead {
     double qs;  // the entries' sum (rest: of q)
     float tm;
-    bool any, far;  // far: a student's logit that Sum does not hold
+    bool any;
 };
 struct EntryRegs {  // as loaded, an entry or two a lane
     int id[2];
@@ -1070,12 +1070,10 @@ __device__ __forceinline__ EntryRegs fetch_entries(const Teacher& Te, long long 
     return e;
 }
 
-template <class T>
-__device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e, const Teacher& Te, float c) {
+__device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e, const Teacher& Te) {
     const int lane = threadIdx.x & 63;
     EntryHead h;
     int id[2];
-    bool far = false;
     h.tm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -1098,16 +1096,13 @@ __device__ __forceinline__ EntryHead load_entries(Entries& E, const EntryRegs& e
         const int j = lane + 64 * u;
         if (64 * u >= Te.k) continue;
         if (j < Te.k) {
-            const float xj = id[u] >= 0 && e.legal[u] ? e.x[u] : -INFINITY;
-            far |= xj != -INFINITY && !(fabsf(xj * c) < FAR);
             E.id[j] = id[u];
             E.t[j] = e.t[u];
-            E.x[j] = xj;
+            E.x[j] = id[u] >= 0 && e.legal[u] ? e.x[u] : -INFINITY;
             E.q[j] = q[u] * iq;
             E.first[j] = true;
         }
     }
-    h.far = __ballot(far) != 0;
     team_sync<64>();
     return h;
 }
@@ -1134,8 +1129,12 @@ __device__ __forceinline__ bool find_repeats(Entries& E, int k) {
 struct Row {  // what the gradient needs of a row: p(x, ref, s) = 2^u(x, ref) / s
     float ro, so, b;  // dx = b p(x, ro, so) w / T, but
     float ra, sa, a;  // dx = (a p(x, ra, sa) - q) w / T at the entries
-    float wide, repeats;
+    int flags;
+    float unused;
 };
+// flags: ro is a logit, ra is (each as Stat's `wide`: entries far from all else have a reference of their own
+// kind); an action is given twice
+constexpr int WIDE_OUT = 1, WIDE_ALL = 2, REPEATS = 4;
 struct RowSums {  // so, sa as summed, for the loss
     double so, sa;
 };
@@ -1157,16 +1156,20 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
             mx = nmax(mx, xj[u]);
         }
         mx = wave_max(mx);
-        Stat<false> e{0.f, 0.0, 0.f, v.wide};
+        Stat<false> e{0.f, 0.0, 0.f, false};
         if (mx != -INFINITY) {
-            e.ref = v.wide ? mx : rintf(mx * R.c);
-            e.s = wave_sum((double)ex2(u_of(xj[0], e.ref, v.wide, R.c)) + (double)ex2(u_of(xj[1], e.ref, v.wide, R.c)));
+            // near 0 the whole number next to max x c; from 2^24 on (a mask's fill, a low temperature) f32 may not hold that,
+            // and what it is off by passes the exponential's range: there the maximum itself
+            e.wide = v.wide || !(fabsf(mx * R.c) < 16777216.f);
+            e.ref = e.wide ? mx : rintf(mx * R.c);
+            e.s = wave_sum((double)ex2(u_of(xj[0], e.ref, e.wide, R.c)) + (double)ex2(u_of(xj[1], e.ref, e.wide, R.c)));
         }
         po = v.s != 0.0 ? 1.0 : 0.0;
-        if (e.s != 0.0 && v.s != 0.0) {
-            all.ref = nmax(e.ref, v.ref);
-            const double se = e.s * (double)ex2(v.wide ? (e.ref - all.ref) * R.c : e.ref - all.ref);
-            const double sv = v.s * (double)ex2(v.wide ? (v.ref - all.ref) * R.c : v.ref - all.ref);
+        if (e.s != 0.0 && v.s != 0.0) {  // the sum of both at the larger reference
+            const double d = place(v.ref, v.wide, R.c) - place(e.ref, e.wide, R.c);
+            const double se = d > 0.0 ? e.s * (double)ex2((float)-d) : e.s;
+            const double sv = d > 0.0 ? v.s : v.s * (double)ex2((float)d);
+            if (!(d > 0.0)) all = e;
             all.s = se + sv;
             po = sv / all.s;
         } else if (e.s != 0.0) {
@@ -1181,8 +1184,8 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
     }
     if (!h.any || all.s == 0.0) S = 0.0, qr = 0.0;
     *sums = RowSums{v.s, all.s};
-    return Row{v.ref, (float)v.s, (float)(S * po - qr), all.ref, (float)all.s, (float)S, v.wide ? 1.f : 0.f,
-               repeats ? 1.f : 0.f};
+    return Row{v.ref, (float)v.s, (float)(S * po - qr), all.ref, (float)all.s, (float)S,
+               (v.wide ? WIDE_OUT : 0) | (all.wide ? WIDE_ALL : 0) | (repeats ? REPEATS : 0), 0.f};
 }
 
 // the row's loss, by one wave, its terms in f64
@@ -1190,7 +1193,7 @@ __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const 
                                         const Row& o, const RowSums& sums) {
     if (!h.any || sums.sa == 0.0) return 0.f;
     const int lane = threadIdx.x & 63;
-    const bool wide = o.wide != 0.f;
+    const bool wide = o.flags & WIDE_ALL;
     const double cd = R.c, ln2 = 0.69314718055994530942;
     // the row's logarithms at once, one a lane: of the sums over all and outside, of the entries' sum, of what is left
     const double qr = 1.0 - h.qs;
@@ -1208,7 +1211,7 @@ __device__ __forceinline__ float row_kl(const Rows& R, const Teacher& Te, const 
     }
     loss = wave_sum(loss);
     if (Te.rest && sums.so != 0.0) {
-        const double d = wide ? ((double)o.ro - (double)o.ra) * cd : (double)o.ro - (double)o.ra;
+        const double d = place(o.ro, o.flags & WIDE_OUT, R.c) - place(o.ra, wide, R.c);
         if (!(qr <= 0.0)) loss += qr * (lane_of(ln, 3) - (d * ln2 + lane_of(ln, 1) - lns));
     }
     return (float)loss;
@@ -1249,12 +1252,12 @@ __device__ __forceinline__ void write_entries(const Rows& R, const Teacher& Te, 
         const int id = E.id[j], i = id - from;
         if (id < 0 || i < 0 || i >= V || (mk && !mk[i])) continue;
         float q = (float)E.q[j];
-        if (o.repeats != 0.f) {  // the same index twice: its entries' probabilities add
+        if (o.flags & REPEATS) {  // the same index twice: its entries' probabilities add
             double all = 0.0;
             for (int e = 0; e < Te.k; ++e) all += E.id[e] == id ? E.q[e] : 0.0;
             q = (float)all;
         }
-        const float p = ex2(u_of(E.x[j], o.ra, o.wide != 0.f, R.c)) * (o.a / o.sa);
+        const float p = ex2(u_of(E.x[j], o.ra, o.flags & WIDE_ALL, R.c)) * (o.a / o.sa);
         d[i] = (T)(o.a == 0.f ? 0.f : (p - q) * g);  // a = 0: a row without a legal action
     }
 }
@@ -1265,7 +1268,7 @@ __device__ __forceinline__ void write_outside(const Rows& R, const Row& o, float
     const float b = o.so == 0.f ? 0.f : o.b * g / o.so;
     if (o.so == 0.f)
         map_row<T, TEAM, false>(x, mk, d, V, nt, [](float, int) { return 0.f; });
-    else if (o.wide != 0.f)
+    else if (o.flags & WIDE_OUT)
         map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int) { return ex2((y - o.ro) * R.c) * b; });
     else
         map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int) { return ex2(__builtin_fmaf(y, R.c, -o.ro)) * b; });
@@ -1302,7 +1305,6 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     __shared__ Entries Es[TEAMS];
     __shared__ Row rows[TEAMS];
     __shared__ RowSums sums[TEAMS];
-    __shared__ bool fars[TEAMS];
     const long long r = team_row<TEAM>();
     if (r >= R.rows) return;
     const T* x = row_ptr<T>(R, r);
@@ -1330,10 +1332,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     if (marked)
         for (int i = tid; i < words; i += TEAM) bits[i] = 0;
     EntryHead h;
-    if (tid < 64) {
-        h = load_entries<T>(E, er, Te, R.c);
-        if (tid == 0) fars[mine] = h.far && Te.rest;
-    }
+    if (tid < 64) h = load_entries(E, er, Te);
     bool repeats = false;
     team_sync<TEAM>();
     if (marked) {
@@ -1381,7 +1380,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
     const Stat<false> v =
-        row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, fars[mine], [&](int i) { return skip.one(i); });
+        row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, [&](int i) { return skip.one(i); });
     if (tid < 64) {
         RowSums both;
         const Row o = row_coefficients(R, Te, E, h, v, repeats, &both);
@@ -1407,7 +1406,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     const Row o = rows[mine];
     const float g = row_weight(R, O, r);
     T* d = (T*)O.dx + r * (long long)V;
-    if (NV > 0 && o.wide == 0.f && o.so != 0.f) {
+    if (NV > 0 && !(o.flags & WIDE_OUT) && o.so != 0.f) {
         const float b = o.b * g / o.so;
         auto write = [&](auto nt) {
 #pragma unroll
@@ -1507,7 +1506,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     if constexpr (JOIN)
         if (tid < P.n) part = P.part[r * P.n + tid];
     if (tid < 64) {
-        h = load_entries<T>(E, fetch_entries<T>(Te, r, R.V, x, mk, JOIN ? 0 : from, JOIN ? R.V : from + V), Te, R.c);
+        h = load_entries(E, fetch_entries<T>(Te, r, R.V, x, mk, JOIN ? 0 : from, JOIN ? R.V : from + V), Te);
         if constexpr (JOIN) repeats = find_repeats(E, Te.k);
     }
     Row o;
@@ -1515,7 +1514,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     if constexpr (JOIN) {
         if (tid < 64) {
             Sum<false> a = part_sum(part);
-            bool again = (Te.rest && h.far) || part.w != 0.f;
+            bool again = part.w != 0.f;
             for (int i = tid + 64; i < P.n; i += 64) {
                 const float4 p = P.part[r * P.n + i];
                 const float m = fmaxf(a.r, p.x);

@@ -37,3 +37,55 @@ def test_teacher_of_one_size():
     loss, d = p.distill_loss_grad(x, low, ids, rest=True, weight=1.0)
     none, dn = p.distill_loss_grad(x, torch.full_like(low, -1e4), ids, rest=True, weight=1.0)
     assert loss.isfinite() and torch.equal(loss, none) and torch.equal(d, dn)
+
+
+FAR = [s * v for v in (1e7, 1e9, 3e9, 1e10, 1e11, 1e12, 1e15, 1e20, 1e29) for s in (1, -1)]
+
+
+@pytest.mark.parametrize("which", ["all", "first", "third"])
+@pytest.mark.parametrize("n,V,dtype", [f for f in FORMS if f[2] != "f16"])
+def test_student_far_at_the_entries(n, V, dtype, which):
+    """The student's logits at all entries, or at one, far above or below all others."""
+    x0 = _logits(n, V, DT[dtype])
+    t, ids = _teacher(x0, 12, None)
+    at = {"all": slice(0, 12), "first": slice(0, 1), "third": slice(2, 3)}[which]
+    rows = torch.arange(n)[:, None]
+    for i, far in enumerate(FAR):
+        x = x0.clone()
+        x[rows, ids[:, at]] = far
+        _check_distill(x, None, t, ids, True)
+        if i % 3 == 0:
+            _check_distill(x, None, t, ids, False)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_student_far_by_temperature(dtype, rest):
+    for n, V in ((5, 343), (130, 20011), (3, 20011)):
+        x = _logits(n, V, DT[dtype])
+        t, ids = _teacher(x, 12, None)
+        for far in (1e4, -1e4, 6e4, -6e4):
+            x[torch.arange(n)[:, None], ids[:, :4]] = far
+            _check_distill(x, None, t, ids, rest, T=1e-6)
+
+
+def test_student_far_at_different_entries():
+    """Entries at the lowest value, some 1e10 above and below, some illegal, none outside, masked outside."""
+    n, V = 8, 343
+    x = _logits(n, V, torch.float32)
+    t, ids = _teacher(x, 10, None)
+    r = torch.arange(n)[:, None]
+    x[r[:4], ids[:4, :5]] = torch.finfo(torch.float32).min
+    x[r[2:6], ids[2:6, 5:7]] = -1e10
+    x[r[3:7], ids[3:7, 7:8]] = 2e10
+    x[7] = -1e10
+    x[7, ids[7, 0]] = -2e10
+    m = torch.rand((n, V), generator=torch.Generator().manual_seed(0)) < 0.5
+    for k in range(10):
+        m[torch.arange(n), ids[:, k]] = True
+    m[1] = False
+    m[1, ids[1]] = True  # nothing outside
+    m[5, ids[5, 7]] = False
+    for mask in (None, m.cuda()):
+        for rest in (False, True):
+            _check_distill(x, mask, t, ids, rest)
