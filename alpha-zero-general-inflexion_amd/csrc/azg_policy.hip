@@ -264,14 +264,21 @@ struct Sum {
 };
 __device__ __forceinline__ float scale2(float x, int k) { return __builtin_amdgcn_ldexpf(x, k); }
 __device__ __forceinline__ double scale2(double x, int k) { return __builtin_amdgcn_ldexp(x, k); }
+// to a reference r >= a.r.  By more than 300, which nothing of a finite sum outlasts, it is set to 0: d s would pass
+// f32 for a sum of fills (-1e9 and the like) although 2^d leaves nothing of it, and so may s.  A NaN stays.
+template <bool ENT>
+__device__ __forceinline__ Sum<ENT> move_sum(Sum<ENT> a, float r) {
+    const float d = a.r - r;
+    const int k = (int)fmaxf(d, -4096.f);
+    const bool gone = d < -300.f && a.s > 0;
+    if constexpr (ENT) a.w = gone ? 0.f : scale2(__builtin_fmaf(d, a.s, a.w), k);
+    a.s = gone ? 0 : scale2(a.s, k);
+    a.r = r;
+    return a;
+}
 template <bool ENT, int N>
 __device__ __forceinline__ void sum_group(Sum<ENT>& a, const float* x, float gm, float c) {
-    if (__builtin_fmaf(gm, c, -a.r) > 8.f) {
-        const float r = rintf(gm * c), d = a.r - r;
-        if constexpr (ENT) a.w = scale2(__builtin_fmaf(d, a.s, a.w), (int)fmaxf(d, -4096.f));
-        a.s = scale2(a.s, (int)fmaxf(d, -4096.f));
-        a.r = r;
-    }
+    if (__builtin_fmaf(gm, c, -a.r) > 8.f) a = move_sum(a, rintf(gm * c));
     float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
@@ -286,13 +293,6 @@ __device__ __forceinline__ void sum_group(Sum<ENT>& a, const float* x, float gm,
     }
     a.s += s0 + s1;
     if constexpr (ENT) a.w += w0 + w1;
-}
-template <bool ENT>
-__device__ __forceinline__ Sum<ENT> move_sum(Sum<ENT> a, float r) {  // to a reference r >= a.r
-    const float d = a.r - r;
-    const int k = (int)fmaxf(d, -4096.f);
-    if constexpr (ENT) a.w = scale2(__builtin_fmaf(d, a.s, a.w), k);
-    return Sum<ENT>{r, scale2(a.s, k), a.w};
 }
 template <int TEAM, bool ENT>
 __device__ __forceinline__ Sum<ENT> team_sum(Sum<ENT> a, Sum<ENT>* sh) {
@@ -380,7 +380,9 @@ __device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2
 }
 // is this sum a row's (some probability, all numbers)?  An empty one is a row without a legal action, or a wide one.
 template <bool ENT>
-__device__ __forceinline__ bool plain_sum(const Sum<ENT>& a) { return a.s > 0.f && a.s < INFINITY; }
+__device__ __forceinline__ bool plain_sum(const Sum<ENT>& a) {
+    return a.s > 0.f && a.s < INFINITY && fabsf(a.w) < INFINITY;
+}
 
 // order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {

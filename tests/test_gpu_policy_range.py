@@ -89,3 +89,22 @@ def test_student_far_at_different_entries():
     for mask in (None, m.cuda()):
         for rest in (False, True):
             _check_distill(x, mask, t, ids, rest)
+
+
+FILLS = [-1e9, -2e9, -1e10]
+
+
+@pytest.mark.parametrize("T", [0.05, 0.2, 0.4, 0.6, 1.0, 1.2, 1.5, 4.0, 5.0])
+@pytest.mark.parametrize("n,V,dtype", [(4, 343, "f32"), (130, 5003, "f32"), (130, 20011, "bf16"), (3, 20011, "f32"),
+                                       (2, 100003, "bf16")])
+def test_fills_leave_the_entropy(n, V, dtype, T):
+    """Legal logits of a mask's fill beside ordinary ones, in turn, in whole stretches of a row, in its last elements:
+    entropy, its gradient and the alternatives."""
+    for fill in FILLS:
+        x = _logits(n, V, DT[dtype])
+        f = torch.tensor(fill).to(x.dtype).item()
+        x[0, ::2] = f
+        x[1, :V // 2] = f
+        x[1, V // 2 + 1:V // 2 + 99] = f
+        x[-1, V // 3:] = f
+        _check_logprobs(x, None, _actions(n, V), 9, T=T)
