@@ -252,8 +252,9 @@ __device__ __forceinline__ double exp_f64(double t) {
 // ---- softmax statistics -------------------------------------------------------------------------
 // s = sum 2^u, w = sum u 2^u with u = x c - r and r a whole number near max x c: moving a sum to another r is exact
 // (a power of two), and x c - r is one rounding.  r follows the maximum lazily (u <= 8.5), and starts at -2^100 with
-// an empty sum.  Where |x c| passes 2^100 (the type's lowest value in f32 and bf16) or a logit is no number, the row
-// is done again by `Soft` below, with u = (x - m) c.
+// an empty sum.  From 2^24 on r is not next to max x c but f32's number next to it: off by up to 8 below 2^28, by more than
+// f32's exponents reach soon after.  A row whose r is at 2^28 or beyond (all its logits at a mask's fill, or one far
+// above the others) or that holds no number is done again by `Soft` below, with u = (x - m) c.
 // ENT: f32 sums with the entropy's; else s alone, in f64 beyond a thread's 16 or 32 terms (a KL is a difference of
 // near values: what s is off by comes to twenty times that of it).
 template <bool ENT>
@@ -378,11 +379,33 @@ __device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2
     if (fabsf(x) > 1e30f) return x * invT - LN2 * (st.ref + l2);  // x c may pass f32 where x / T does not
     return LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
 }
-// is this sum a row's (some probability, all numbers)?  An empty one is a row without a legal action, or a wide one.
+// is this sum a row's (some probability, all numbers, at a reference near its maximum: then s >= 2^-8, and s and w are
+// finite)?  An empty one is a row without a legal action, or a wide one.
 template <bool ENT>
 __device__ __forceinline__ bool plain_sum(const Sum<ENT>& a) {
-    return a.s > 0.f && a.s < INFINITY && fabsf(a.w) < INFINITY;
+    return a.s > 0.f && a.s < INFINITY && fabsf(a.r) < 268435456.f;
 }
+
+// The parts of a row that is split over blocks: (r, s, w or s in two words, kind).  A part that Sum does not hold
+// leaves s = 0 and its maximum's x c in place of r; where that is far below the other parts' r (a stretch of fills) the
+// part counts for nothing, else the row is done again.
+constexpr float PART_SUM = 0.f, PART_FAR = 1.f, PART_AGAIN = 2.f;  // PART_AGAIN: some logit is no number
+__device__ __forceinline__ float part_kind(bool plain, float max) {
+    return plain || max == -INFINITY ? PART_SUM : fabsf(max) < INFINITY ? PART_FAR : PART_AGAIN;
+}
+struct FarParts {
+    float top = -INFINITY;
+    bool any = false, again = false;
+    __device__ __forceinline__ void add(float4 p) {
+        any = true;
+        again |= p.w == PART_AGAIN;
+        top = fmaxf(top, p.x * (p.x < 0.f ? 1.f - 0x1p-22f : 1.f + 0x1p-22f));  // x c is rounded, and so may r be
+    }
+    template <bool ENT>
+    __device__ __forceinline__ bool redo(const Sum<ENT>& a) const {
+        return any && (again || !(a.s > 0 && top < a.r - 300.f));
+    }
+};
 
 // order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {
@@ -789,7 +812,7 @@ __device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, l
     }
 }
 
-// a part of a row for rows split over blocks: (r, s, w, 1 if it has to be done again as a wide row)
+// rows split over blocks
 struct Split {
     float4* part;               // [rows][n]
     unsigned long long* keys;   // [rows][n][k], by rank, 0: none
@@ -823,20 +846,25 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
     row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{}, r < O.keep);
     Stat<true> st;
     float l2 = 0.f;
+    bool numbers;  // no NaN, no +inf: the alternatives by their bound
     if constexpr (PART) {
         a = team_sum<TEAM, true>(a, sh.sum);
         const bool plain = plain_sum(a);
-        const float all = plain ? 0.f : team_max<TEAM>(mx, sh.f);
-        st.wide = !plain && all != -INFINITY;
-        if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(a.r, plain ? a.s : 0.f, plain ? a.w : 0.f, st.wide);
+        const float all = plain ? 0.f : team_max<TEAM>(mx, sh.f), kind = part_kind(plain, all);
+        numbers = kind != PART_AGAIN;
+        if (tid == 0)
+            P.part[r * P.n + blockIdx.z] = plain                ? make_float4(a.r, a.s, a.w, kind)
+                                           : kind == PART_SUM ? make_float4(-FAR, 0.f, 0.f, kind)
+                                                                : make_float4(all * R.c, 0.f, 0.f, kind);
     } else {
         st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, [](int) { return false; });
         l2 = lg2(st.s);
+        numbers = st.s == st.s;
         if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
     }
     if constexpr (TOP) {
         TopShare<TEAM>& S = tops[team_in_block<TEAM>()];
-        const int n = top_select<T, TEAM, MASK>(x, mk, V, O.k, !st.wide, best, gmax, S);
+        const int n = top_select<T, TEAM, MASK>(x, mk, V, O.k, numbers, best, gmax, S);
         top_out<TEAM>(S, n, O.k, [&](int rank, unsigned long long key) {
             if constexpr (PART) {
                 // the index within the row: the key holds its complement
@@ -862,15 +890,18 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
     const int tid = threadIdx.x;
     const long long act = action_of(O, r);
     Sum<true> a{-FAR, 0.f, 0.f};
-    bool again = false;
+    FarParts far;
     for (int i = tid; i < P.n; i += 256) {
         const float4 p = P.part[r * P.n + i];
+        if (p.w != PART_SUM) {
+            far.add(p);
+            continue;
+        }
         const float m = fmaxf(a.r, p.x);
         const Sum<true> b = move_sum(Sum<true>{p.x, p.y, p.z}, m);
         a = move_sum(a, m);
         a.s += b.s;
         a.w += b.w;
-        again |= p.w != 0.f;
     }
     unsigned long long best = 0;
     const unsigned long long* keys = nullptr;
@@ -879,14 +910,11 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
         keys = P.keys + r * nk;
         for (int i = tid; i < nk; i += 256) best = best > keys[i] ? best : keys[i];
     }
-    again = __syncthreads_or(again);
-    Stat<true> st;
-    if (again) {
+    a = team_sum<256, true>(a, sh.sum);
+    Stat<true> st{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
+    if (__syncthreads_or(far.redo(a))) {
         const Soft v = soft_pass<T, 256>(x, mk, R.V, R.c, sh.soft, [](int) { return false; });
         st = Stat<true>{v.m, v.s, v.w, true};
-    } else {
-        a = team_sum<256, true>(a, sh.sum);
-        st = Stat<true>{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
     }
     const float l2 = lg2(st.s);
     if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
@@ -1440,7 +1468,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
     loss();  // last: the other waves do not wait for it
 }
 
-// a part of a row of few rows: its statistics outside the entries, as (r, s in two words, 1 if the row is a wide one)
+// a part of a row of few rows: its statistics outside the entries
 __device__ __forceinline__ Sum<false> part_sum(float4 p) {
     const unsigned long long w = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.y);
     return Sum<false>{p.x, __longlong_as_double((long long)w), 0.f};
@@ -1476,11 +1504,11 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
     row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     a = team_sum<256, false>(a, sh.sum);
     const bool plain = plain_sum(a);
-    const bool again = !plain && team_max<256>(mx, sh.f) != -INFINITY;
+    const float all = plain ? 0.f : team_max<256>(mx, sh.f), kind = part_kind(plain, all);
     if (tid == 0) {
         const unsigned long long w = (unsigned long long)__double_as_longlong(plain ? a.s : 0.0);
-        P.part[r * P.n + blockIdx.z] =
-            make_float4(a.r, __uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)), again);
+        P.part[r * P.n + blockIdx.z] = make_float4(plain ? a.r : kind == PART_SUM ? -FAR : all * R.c,
+                                                   __uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)), kind);
     }
 }
 
@@ -1504,7 +1532,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     Entries& E = Es[team_in_block<TEAM>()];
     EntryHead h;
     bool repeats = false;
-    float4 part{-FAR, 0.f, 0.f, 0.f};  // ahead of the entries: their loads wait for each other
+    float4 part{-FAR, 0.f, 0.f, PART_SUM};  // ahead of the entries: their loads wait for each other
     if constexpr (JOIN)
         if (tid < P.n) part = P.part[r * P.n + tid];
     if (tid < 64) {
@@ -1515,18 +1543,19 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     RowSums sums;
     if constexpr (JOIN) {
         if (tid < 64) {
-            Sum<false> a = part_sum(part);
-            bool again = part.w != 0.f;
-            for (int i = tid + 64; i < P.n; i += 64) {
-                const float4 p = P.part[r * P.n + i];
+            Sum<false> a{-FAR, 0.0, 0.f};
+            FarParts far;
+            auto join = [&](float4 p) {
+                if (p.w != PART_SUM) return far.add(p);
                 const float m = fmaxf(a.r, p.x);
                 const Sum<false> b = move_sum(part_sum(p), m);
                 a = move_sum(a, m);
                 a.s += b.s;
-                again |= p.w != 0.f;
-            }
+            };
+            join(part);
+            for (int i = tid + 64; i < P.n; i += 64) join(P.part[r * P.n + i]);
             a = team_sum<64, false>(a, nullptr);
-            again = __ballot(again) != 0;
+            const bool again = __ballot(far.redo(a)) != 0;
             if (tid == 0) joined = Stat<false>{a.s > 0.0 ? a.r : 0.f, a.s, 0.f, again};
         }
         __syncthreads();

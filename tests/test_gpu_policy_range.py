@@ -108,3 +108,45 @@ def test_fills_leave_the_entropy(n, V, dtype, T):
         x[1, V // 2 + 1:V // 2 + 99] = f
         x[-1, V // 3:] = f
         _check_logprobs(x, None, _actions(n, V), 9, T=T)
+
+
+@pytest.mark.parametrize("fill", [2.4e8, 1e9, 1.5e9, 1.6e9, -2e9, 2.2e9, -2.5e9, 2.9e9, -5e9, 1e10, -3e20])
+@pytest.mark.parametrize("n,V,dtype", [(4, 343, "f32"), (6, 1001, "bf16"), (130, 5003, "f32"), (130, 20011, "f32"),
+                                       (3, 20011, "f32"), (2, 100003, "bf16")])
+def test_rows_of_one_large_value(n, V, dtype, fill):
+    """Rows whose largest logit is far from 0: probabilities, entropy and the gradients with incoming ones of a loss scale."""
+    p = _policy()
+    x = torch.full((n, V), fill).to(DT[dtype]).cuda()
+    x[0, ::3] = torch.finfo(DT[dtype]).min
+    x[1, 1::2] = -1e30
+    _check_logprobs(x, None, _actions(n, V), 5)
+    t, ids = _teacher(_logits(n, V, torch.float32), 6, None)
+    ids[0, :3] = torch.tensor([1, 4, 7])
+    for rest in (False, True):
+        _check_distill(x, None, t, ids, rest)
+        loss, tol, d, dd = po.distill(x, t, ids, None, 1.0, rest)
+        for w in (2.0 ** 16, 2.0 ** -20):
+            _, g = p.distill_loss_grad(x, t.cuda(), ids.cuda(), rest=rest, weight=w)
+            one = torch.full((1, 1), w, dtype=torch.float64, device="cuda")
+            po.check(g, d * one, po.grad_tol(d, dd, one, x.dtype), f"gradient of {w} times the sum")
+    for w in (2.0 ** 16, 2.0 ** -20):
+        leaf = x.clone().requires_grad_(True)
+        g1 = torch.full((n,), w)
+        q = p.action_logprobs(leaf, _actions(n, V).cuda())
+        d, = torch.autograd.grad((q.logp, q.entropy), leaf, (g1.cuda(), g1.cuda()))
+        po.check(d, *po.logprobs_grad(x, _actions(n, V), None, 1.0, g1, g1, None), f"gradient of {w} logp and entropy")
+
+
+@pytest.mark.parametrize("T", [0.05, 0.2, 0.6, 1.2, 4.0])
+@pytest.mark.parametrize("n,V,dtype", [(4, 343, "f32"), (130, 5003, "f32"), (3, 20011, "f32"), (2, 100003, "bf16")])
+def test_large_values_at_temperatures(n, V, dtype, T):
+    """Ordinary logits beside stretches of a large value, as the row's largest or its smallest."""
+    for fill in (3e8, 1e9, 2e9, 3e9, -2e9):
+        x = _logits(n, V, DT[dtype])
+        x[0, ::2] = fill
+        x[1, :V // 2] = fill
+        x[-1, V // 3:] = fill
+        _check_logprobs(x, None, _actions(n, V), 9, T=T)
+        t, ids = _teacher(_logits(n, V, torch.float32, seed=1), 9, None)
+        _check_distill(x, None, t, ids, True, T=T)
+        _check_distill(x, None, t, ids, False, T=T)
