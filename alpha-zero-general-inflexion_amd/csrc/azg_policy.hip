@@ -193,13 +193,13 @@ __device__ __forceinline__ void store16(T* p, const float* f) {
     else
         *(W*)p = w;
 }
-// illegal actions of a vector -> -inf
+// illegal actions of a vector -> none
 template <class T>
-__device__ __forceinline__ void apply_mask(const uint8_t* mk, float* f) {
+__device__ __forceinline__ void apply_mask(const uint8_t* mk, float* f, float none = -INFINITY) {
     uint8_t b[VN<T>];
     __builtin_memcpy(b, mk, VN<T>);
 #pragma unroll
-    for (int i = 0; i < VN<T>; ++i) f[i] = b[i] ? f[i] : -INFINITY;
+    for (int i = 0; i < VN<T>; ++i) f[i] = b[i] ? f[i] : none;
 }
 
 // 1 / x for x in the normal range: the instruction's estimate (2^-24 or better) and two Newton steps, which square its
@@ -1447,9 +1447,9 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
                     if ((q * U + u) * TEAM >= nvec || vi >= nvec) continue;
                     float y[N];
                     unpack<T>(L[q].v[u], y);
-                    if constexpr (MASK) apply_mask<T>(mk + vi * N, y);
 #pragma unroll
                     for (int i = 0; i < N; ++i) y[i] = ex2(__builtin_fmaf(y[i], R.c, -o.ro)) * b;
+                    if constexpr (MASK) apply_mask<T>(mk + vi * N, y, 0.f);  // not before: b may be no number
                     store16<decltype(nt)::value>(d + (long long)vi * N, y);
                     __builtin_amdgcn_sched_barrier(0);
                 }

@@ -150,3 +150,29 @@ def test_large_values_at_temperatures(n, V, dtype, T):
         t, ids = _teacher(_logits(n, V, torch.float32, seed=1), 9, None)
         _check_distill(x, None, t, ids, True, T=T)
         _check_distill(x, None, t, ids, False, T=T)
+
+
+@pytest.mark.parametrize("n,V,dtype", FORMS)
+def test_illegal_actions_get_no_gradient(n, V, dtype):
+    """A teacher's NaN, and weights that are no finite numbers, leave 0 at the illegal actions of their rows."""
+    p = _policy()
+    x = _logits(n, V, DT[dtype])
+    m = _mask("random", n, V)
+    t, ids = _teacher(x, 12, m)
+    t[0, 1] = math.nan
+    t, ids = t.cuda(), ids.cuda()
+    w = torch.ones(n, device="cuda")
+    w[-1] = math.inf
+    w[1] = math.nan
+    for rest in (False, True):
+        _, g = p.distill_loss_grad(x, t, ids, mask=m, rest=rest, weight=w)
+        leaf = x.clone().requires_grad_(True)
+        rows = p.distill_loss(leaf, t, ids, mask=m, rest=rest, reduction="none")
+        d, = torch.autograd.grad(rows, leaf, w)
+        for q in (g, d):
+            assert (q[~m] == 0).all()
+            assert q[1][m[1]].isnan().all()
+            if rest:
+                assert q[0][m[0]].isnan().all()
+            if n > 3:
+                assert q[2][m[2]].isfinite().all()
