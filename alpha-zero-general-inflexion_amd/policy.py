@@ -16,13 +16,14 @@ broadcasts to it, bool or uint8) marks the legal actions: what stands at an ille
 number (infinities and NaN there do not matter), its probability and its gradient are 0.  A legal
 logit of -inf is probability 0; a legal NaN or +inf makes its row's numbers NaN.  All work is queued on
 the current stream of the logits' device; nothing synchronises, and results do not depend on the
-order in which blocks run."""
+order in which blocks run.  Gradients are those of reverse mode, once; a forward-mode tangent is refused."""
 import functools
 import math
 import struct
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -85,6 +86,15 @@ def _check_logits(name, logits, temperature):
     if not (1e-6 <= t <= 1e6):
         raise ValueError(f"{name}: temperature {temperature} (1e-6 to 1e6)")
     return t
+
+
+def _check_tangents(name, *tensors):
+    """The kernels read values alone: a tangent would be dropped."""
+    if forward_ad._current_level < 0:  # outside of dual_level(), the usual case
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _check_mask(name, logits, mask):
@@ -208,6 +218,7 @@ class _ActionLogprobs(torch.autograd.Function):
         logits, mask, actions, stats = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_lse is None:
             return None, None, None, None, None
+        _check_tangents("action_logprobs' gradient", g_logp, g_entropy, g_lse)
         logits, mask, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if n:
@@ -232,6 +243,7 @@ def action_logprobs(logits, actions=None, *, top=0, temperature=1.0, mask=None):
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(TOP_MAX, logits.shape[-1]):
         raise ValueError(f"action_logprobs: top = {top!r} (an int from 0 to min({TOP_MAX}, V = {logits.shape[-1]}))")
     mask = _check_mask("action_logprobs", logits, mask)
+    _check_tangents("action_logprobs", logits)
     if actions is not None:
         actions = _check_ints("action_logprobs", "actions", actions, logits.shape[:-1], logits.device)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -250,6 +262,7 @@ def _check_teacher(name, logits, teacher_logp, teacher_ids):
         raise ValueError(f"{name}: teacher_logp on {teacher_logp.device}, logits on {logits.device}")
     if teacher_logp.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: the teacher gets no gradient: detach teacher_logp")
+    _check_tangents(name, logits, teacher_logp)
     ids = _check_ints(name, "teacher_ids", teacher_ids, teacher_logp.shape, logits.device)
     if teacher_logp.requires_grad:
         teacher_logp = teacher_logp.detach()
@@ -295,6 +308,7 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, mask, t_logp, t_ids, stats = ctx.saved_tensors
+        _check_tangents("distill_loss's gradient", g)
         logits, mask, n, L = _rows(logits, mask, ctx.t)
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if n:
@@ -350,6 +364,7 @@ def distill_loss_grad(logits, teacher_logp, teacher_ids, *, temperature=1.0, mas
         if weight.dim() and weight.shape != logits.shape[:-1]:
             raise ValueError(f"distill_loss_grad: weight {tuple(weight.shape)}, expected "
                              f"{tuple(logits.shape[:-1])} or one number")
+        _check_tangents("distill_loss_grad", weight)
         w = weight.detach()
     else:
         scale = float(weight)

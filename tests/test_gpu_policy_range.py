@@ -176,3 +176,30 @@ def test_illegal_actions_get_no_gradient(n, V, dtype):
                 assert q[0][m[0]].isnan().all()
             if n > 3:
                 assert q[2][m[2]].isfinite().all()
+
+
+def test_forward_mode_is_refused():
+    """No forward-mode derivative: a tangent is refused rather than dropped."""
+    from torch.autograd import forward_ad as fwd
+    p = _policy()
+    x = _logits(4, 65, torch.float32)
+    a = _actions(4, 65).cuda()
+    t, ids = _teacher(x, 5, None)
+    t, ids = t.cuda(), ids.cuda()
+    w = torch.ones(4, device="cuda")
+    with fwd.dual_level():
+        dx, dt, dw = (fwd.make_dual(q, torch.ones_like(q)) for q in (x, t, w))
+        for bad in (lambda: p.action_logprobs(dx, a), lambda: p.distill_loss(dx, t, ids),
+                    lambda: p.distill_loss(x, dt, ids), lambda: p.distill_loss_grad(dx, t, ids),
+                    lambda: p.distill_loss_grad(x, dt, ids), lambda: p.distill_loss_grad(x, t, ids, weight=dw)):
+            with pytest.raises(RuntimeError, match="forward"):
+                bad()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+            p.action_logprobs(dx, a)
+        leaf = x.clone().requires_grad_(True)  # a tangent of what reaches the results
+        for y in (p.action_logprobs(leaf, a).entropy, p.distill_loss(leaf, t, ids, reduction="none")):
+            with pytest.raises(RuntimeError, match="forward"):
+                torch.autograd.grad((y * dw).sum(), leaf)
+        want = p.action_logprobs(x, a).logp  # no tangent: as outside
+        assert torch.equal(p.action_logprobs(dx.detach(), a).logp, want)
+    assert torch.equal(p.action_logprobs(x, a).logp, want)
