@@ -179,15 +179,16 @@ def _logprobs(logits, actions, top, t, mask, want_stats):
     lead, dev = logits.shape[:-1], logits.device
     logits, mask, n, L = _rows(logits, mask, t)
     logp = top_logp = top_ids = stats = None
-    if want_stats:  # tensors of their own: autograd lets nobody write into views that a Function returns
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        lse = torch.empty(lead, dtype=torch.float32, device=dev)
-        if actions is not None:
-            logp = torch.empty(lead, dtype=torch.float32, device=dev)
-    elif actions is None:
-        entropy, lse = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind(0)
+    # One allocation, but tensors of their own: to autograd unsafe_chunk's results are no views, so they may be written
+    # with what requires a gradient, and a write to one is none to the others (three allocations: 1.1 to 3.1 us more)
+    c = 2 if actions is None else 3
+    if lead:
+        rows = torch.unsafe_chunk(torch.empty((c * lead[0], *lead[1:]), dtype=torch.float32, device=dev), c)
     else:
-        entropy, lse, logp = torch.empty((3, *lead), dtype=torch.float32, device=dev).unbind(0)
+        rows = [torch.empty((), dtype=torch.float32, device=dev) for _ in range(c)]
+    entropy, lse = rows[:2]
+    if c == 3:
+        logp = rows[2]
     if top:
         top_logp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
         top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)

@@ -203,3 +203,33 @@ def test_forward_mode_is_refused():
         want = p.action_logprobs(x, a).logp  # no tangent: as outside
         assert torch.equal(p.action_logprobs(dx.detach(), a).logp, want)
     assert torch.equal(p.action_logprobs(x, a).logp, want)
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_results_without_a_graph_are_separate(given):
+    """Each result is a tensor of its own: written with what requires a gradient, and without touching the others' graph."""
+    p = _policy()
+    x = _logits(6, 65, torch.float32)
+    w = torch.full((6,), 2.0, device="cuda", requires_grad=True)
+    r = p.action_logprobs(x, _actions(6, 65).cuda() if given else None)
+    plain = [q.clone() for q in r if q is not None]
+    assert len(plain) == 2 + given and not any(q._is_view() for q in r if q is not None)
+    loss = (w * r.entropy).sum()  # entropy is kept for w's gradient
+    r.lse.mul_(w)
+    if given:
+        r.logp.mul_(w)
+    assert r.lse.requires_grad and not r.entropy.requires_grad and r.entropy._version == 0
+    g, = torch.autograd.grad(loss, w)
+    assert torch.equal(g, r.entropy) and torch.equal(r.entropy, plain[-2])
+    g, = torch.autograd.grad(r.lse.sum(), w)
+    assert torch.equal(g, plain[-1])
+    with torch.no_grad():
+        q = p.action_logprobs(x)
+    q.entropy.mul_(w)
+    assert q.entropy.requires_grad
+    for shape in ((65,), (0, 65), (2, 0, 65), (2, 3, 65)):  # one row, none, several leading dimensions
+        y = _logits(6, 65, torch.float32).reshape(2, 3, 65)
+        y = y[0, 0] if len(shape) == 1 else y if 0 not in shape else y.new_empty(shape)
+        a = torch.zeros(shape[:-1], dtype=torch.int64, device="cuda") if given else None
+        r = p.action_logprobs(y, a)
+        assert all(q.shape == shape[:-1] and q.is_contiguous() for q in r if q is not None)
