@@ -373,11 +373,17 @@ __device__ __forceinline__ float u_of(float x, float ref, bool wide, float c) {
 }
 // the reference in units of x c (48 bits of a product: exact)
 __device__ __forceinline__ double place(float ref, bool wide, float c) { return wide ? (double)ref * (double)c : ref; }
-// the log-probability of a logit, l2 = log2 of the row's sum
+// the log-probability of a logit, l2 = log2 of the row's sum: a difference of near values for a nearly sure policy,
+// which rounding leaves above 0 now and then.  A NaN stays.
 __device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2, float c, float invT) {
-    if (st.wide) return (x - st.ref) * invT - LN2 * l2;
-    if (fabsf(x) > 1e30f) return x * invT - LN2 * (st.ref + l2);  // x c may pass f32 where x / T does not
-    return LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
+    float p;
+    if (st.wide)
+        p = (x - st.ref) * invT - LN2 * l2;
+    else if (fabsf(x) > 1e30f)
+        p = x * invT - LN2 * (st.ref + l2);  // x c may pass f32 where x / T does not
+    else
+        p = LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
+    return p > 0.f ? 0.f : p;
 }
 // is this sum a row's (some probability, all numbers, at a reference near its maximum: then s >= 2^-8, and s and w are
 // finite)?  An empty one is a row without a legal action, or a wide one.
@@ -798,7 +804,8 @@ template <class T>
 __device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, long long r, const Stat<true>& st,
                                           float l2, long long act, const T* x, const uint8_t* mk) {
     const bool empty = st.s == 0.f;
-    const float H = empty ? 0.f : LN2 * (l2 - st.w / st.s);
+    float H = empty ? 0.f : LN2 * (l2 - st.w / st.s);
+    if (H < 0.f) H = 0.f;  // a difference of near values, as logp_of's; a NaN stays
     if (O.stats) ((float4*)O.stats)[r] = make_float4(st.ref, st.s, H, st.wide ? 1.f : 0.f);
     O.entropy[r] = H;
     O.lse[r] = empty ? -INFINITY : st.wide ? st.ref * R.invT + LN2 * l2 : LN2 * (st.ref + l2);

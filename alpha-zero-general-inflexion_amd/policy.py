@@ -235,7 +235,7 @@ def action_logprobs(logits, actions=None, *, top=0, temperature=1.0, mask=None):
 
     actions [...] (int64 or int32; None: no logp): one per row; an action outside 0..V-1 (padding) has
     log-probability 0 and no gradient, an illegal one -inf.  Returns ActionLogprobs:
-      logp, entropy, lse [...]   f32; lse = log sum exp(logits / temperature); differentiable
+      logp, entropy, lse [...]   f32; lse = log sum exp(logits / temperature); differentiable; logp <= 0 <= entropy
       top_logp, top_ids [..., top]  f32 / int64 (None when top = 0), likeliest first, equal logits in
                                  the order of their indices; not differentiable
     A row with fewer than `top` legal actions of probability above 0 is filled up with -inf and -1; one without any

@@ -233,3 +233,23 @@ def test_results_without_a_graph_are_separate(given):
         a = torch.zeros(shape[:-1], dtype=torch.int64, device="cuda") if given else None
         r = p.action_logprobs(y, a)
         assert all(q.shape == shape[:-1] and q.is_contiguous() for q in r if q is not None)
+
+
+@pytest.mark.parametrize("n,V,dtype", FORMS)
+def test_no_probability_above_one(n, V, dtype):
+    """Nearly sure policies: log-probabilities are never above 0, entropies never below."""
+    p = _policy()
+    for sure in (12.0, 17.0, 20.0, 30.0, 100.0):
+        x = _logits(n, V, DT[dtype])
+        a = torch.arange(n) % V
+        x[torch.arange(n), a] += sure
+        r = p.action_logprobs(x, a.cuda(), top=3)
+        assert (r.logp <= 0).all() and (r.top_logp <= 0).all() and (r.entropy >= 0).all()
+        _check_logprobs(x, None, a, 3)
+    # One action: s = 2^u, |u| <= 1/2.  With h = 2^-24 the exponential is off by 2 h of itself, its logarithm by 2 h / ln 2
+    # for that and by a step of the instruction (h), u - log2 s is exact, and u s / s adds 3 roundings of at most h / 2: times
+    # ln 2 under 4 h.
+    x = _logits(n, V, torch.float32)[:, :1]
+    r = p.action_logprobs(x, torch.zeros(n, dtype=torch.int64, device="cuda"), top=1)
+    for q in (-r.logp, -r.top_logp, r.entropy):
+        assert (q >= 0).all() and (q < 4 * po.H).all()
