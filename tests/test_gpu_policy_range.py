@@ -253,3 +253,83 @@ def test_no_probability_above_one(n, V, dtype):
     r = p.action_logprobs(x, torch.zeros(n, dtype=torch.int64, device="cuda"), top=1)
     for q in (-r.logp, -r.top_logp, r.entropy):
         assert (q >= 0).all() and (q < 4 * po.H).all()
+
+
+def _tight(kind):
+    """policy_oracle.row_slack by what the kernels add, h = 2^-24 an addition.  A term passes at most 16 additions within
+    its thread's group of 16 or 32 logits (two chains), 2 more into the thread's sum, one for each further group (V / 4096
+    of them in a block that takes a whole row: 32 at 131072), 5 for the last group's vectors and the remainder, 6 and 4 in
+    the wave and the block, 12 where parts are joined; the exponential is off by 2 h and 4 h |u|, the logarithm by 2 h of
+    itself.  A KL leaves f32 behind the thread's group, and its logarithms are f64: 18 additions, the conversion to
+    f32 for the gradient, the exponential."""
+    def slack(z, p):
+        V = z.shape[1]
+        u = (z.max(1, keepdim=True).values - z) / math.log(2.0)
+        eu = (p * torch.where(torch.isfinite(u), u, torch.zeros_like(u))).sum(1)
+        if kind == "kl":
+            return po.H * (22 + 4 * eu), eu
+        return po.H * (47 + min(V // 4096, 32) + 4 * eu + 2 * math.log1p(V)), eu
+    return slack
+
+
+ENDS = [(6, 343, "f32"), (6, 343, "bf16"), (6, 1001, "f16"), (2100, 3001, "f32"), (130, 5003, "f32"), (130, 5003, "bf16"),
+        (130, 20011, "f16"), (130, 40001, "f32"), (130, 70001, "bf16"), (128, 131071, "f16"), (4, 20011, "f32"),
+        (3, 100003, "bf16"), (2, 262147, "f32")]
+
+
+@pytest.mark.parametrize("n,V,dtype", ENDS)
+def test_every_element_counts(n, V, dtype, monkeypatch):
+    """A row's mass in the elements behind its last vector, in its last and first vectors, next to the bounds of
+    groups and parts, in one element in a thousand; and equal logits, of which none may be left out."""
+    g = torch.Generator().manual_seed(V)
+    x = _logits(n, V, DT[dtype])
+    near = torch.arange(0, V + 1024, 1024)
+    near = torch.cat([near - 1, near, near + 1])
+    places = [torch.arange(V - V % 8, V), torch.arange(max(0, V - 70), V), torch.arange(min(9, V)), near[(near >= 0) & (near < V)],
+              torch.randint(0, V, (max(1, V // 1000),), generator=g), torch.arange(V - V % 4, V)]
+    for r in range(n):
+        if r % 8 == 7:
+            x[r] = 0.5
+        else:
+            at = places[(r + V) % len(places) if n > 6 else (r + V // 2) % len(places)]
+            x[r, at] = (11.0 + torch.randn(len(at), generator=g)).to(x.dtype).cuda()
+    if n < 8:
+        x = torch.cat([x, torch.full_like(x[:1], 0.5)])
+        n += 1
+    monkeypatch.setattr(po, "row_slack", _tight("logp"))
+    for top in (0, 20):
+        _check_logprobs(x, None, _actions(n, V), top, grads=top == 0)
+    _check_logprobs(x, _mask("random", n, V), _actions(n, V), 9)
+    monkeypatch.setattr(po, "row_slack", _tight("kl"))
+    t, ids = _teacher(x, 12, None)
+    ids[:, 1::2] = torch.randint(0, V, ids[:, 1::2].shape, generator=g)  # half of the mass outside the entries
+    for rest in (False, True):
+        _check_distill(x, None, t, ids, rest)
+        _check_distill(x, _mask("random", n, V), t, ids, rest)
+
+
+@pytest.mark.parametrize("n,V,dtype", ENDS)
+def test_kl_of_near_distributions(n, V, dtype):
+    """Logits whose exponentials are powers of two (the temperature makes log2(e) / T one in f32): 20 entries of 1, all else
+    2^-14 to 2^-20.  A thread's sum of 32 is exact in f32 (24 bits hold up to 16 of the ones), a row's in f64 alone: added up in
+    f32 it would be off by some 3e-8 of itself, and the KL by as much.  Exponentials and logarithms in f64 are good to 1e-11,
+    what remains is the KL's own rounding (0.21 at most)."""
+    p = _policy()
+    T = math.log2(math.e)
+    g = torch.Generator().manual_seed(V)
+    x = -torch.randint(14, 21, (n, V), generator=g).float()
+    ids = (torch.arange(20) * (V // 20) + torch.arange(n)[:, None] % (V // 20)).contiguous()
+    x.scatter_(1, ids, 0.0)
+    t = torch.log_softmax(x.double() / T, 1).gather(1, ids).float()
+    x = x.to(DT[dtype]).cuda()
+    for rest in (False, True):
+        loss, _, _, _ = po.distill(x, t, ids, None, T, rest)
+        assert loss.abs().max() < 0.21  # ln(1 + 262147 * 1.74e-5 / 20)
+        tol = 1e-10 + po.H * loss.abs()
+        got = p.distill_loss(x, t.cuda(), ids.cuda(), rest=rest, temperature=T, reduction="none").double()
+        assert ((got - loss).abs() <= tol).all()
+        one, _ = p.distill_loss_grad(x, t.cuda(), ids.cuda(), rest=rest, temperature=T, weight=1.0)
+        assert abs(one.double() - loss.sum()) <= tol.sum() + po.H * loss.sum().abs()
+        rows = p.distill_loss(x.clone().requires_grad_(True), t.cuda(), ids.cuda(), rest=rest, temperature=T,
+                              reduction="none").double()
+        assert ((rows - loss).abs() <= tol).all()
