@@ -1164,7 +1164,7 @@ __device__ __forceinline__ bool find_repeats(Entries& E, int k) {
 }
 
 struct Row {  // what the gradient needs of a row: p(x, ref, s) = 2^u(x, ref) / s
-    float ro, so, b;  // dx = b p(x, ro, so) w / T, but
+    float ro, so, b;  // dx = b p(x, ro, so) w / T (so = 0: 0, whatever the logits are), but
     float ra, sa, a;  // dx = (a p(x, ra, sa) - q) w / T at the entries
     int flags;
     float unused;
@@ -1219,8 +1219,8 @@ __device__ __forceinline__ Row row_coefficients(const Rows& R, const Teacher& Te
         if (qr < 0.0) qr = 0.0;
         S += qr;
     }
-    if (!h.any || all.s == 0.0) S = 0.0, qr = 0.0;
     *sums = RowSums{v.s, all.s};
+    if (!h.any || all.s == 0.0) return Row{0.f, 0.f, 0.f, 0.f, 1.f, 0.f, 0, 0.f};  // no entry or no legal action
     return Row{v.ref, (float)v.s, (float)(S * po - qr), all.ref, (float)all.s, (float)S,
                (v.wide ? WIDE_OUT : 0) | (all.wide ? WIDE_ALL : 0) | (repeats ? REPEATS : 0), 0.f};
 }

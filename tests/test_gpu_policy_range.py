@@ -333,3 +333,28 @@ def test_kl_of_near_distributions(n, V, dtype):
         rows = p.distill_loss(x.clone().requires_grad_(True), t.cuda(), ids.cuda(), rest=rest, temperature=T,
                               reduction="none").double()
         assert ((rows - loss).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("n,V,dtype", FORMS)
+def test_rows_without_an_entry_get_no_gradient(n, V, dtype, rest):
+    """Padding: no entry, and logits that are no numbers.  Loss 0 and gradient 0, the other rows' as without them."""
+    p = _policy()
+    x = _logits(n, V, DT[dtype])
+    t, ids = _teacher(x, 12, None)
+    m = _mask("random", n, V)
+    t, ids, pad = t.cuda(), ids.cuda(), slice(n - 1, n) if n < 3 else slice(1, n, 3)
+    ids[pad] = -1
+    t[n - 1] = -math.inf
+    y = x.clone()
+    y[pad] = math.nan
+    y[n - 1, V // 2:] = math.inf
+    for mask in (None, m):
+        want, dwant = p.distill_loss_grad(x, t, ids, mask=mask, rest=rest, weight=1.0)
+        for z in (x, y):
+            loss, d = p.distill_loss_grad(z, t, ids, mask=mask, rest=rest, weight=1.0)
+            assert torch.equal(loss, want) and torch.equal(d, dwant) and (d[pad] == 0).all() and (d[n - 1] == 0).all()
+            leaf = z.clone().requires_grad_(True)
+            rows = p.distill_loss(leaf, t, ids, mask=mask, rest=rest, reduction="none")
+            e, = torch.autograd.grad(rows.sum(), leaf)
+            assert (rows[pad] == 0).all() and rows[n - 1] == 0 and (e[pad] == 0).all() and (e[n - 1] == 0).all()
