@@ -1031,7 +1031,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_bwd_kernel(Rows R, co
     const float c0 = (g3 - g1 - g2 * H) * R.invT / s + c1 * lg2(s);
     T* d = dx + r * (long long)R.V + from;
     const int mine = given ? (int)(a - from) : -1;  // outside this part: no element's index
-    if (s == 0.f) {  // no legal action
+    if (s == 0.f || (!given && !ge && !gz)) {  // no legal action, or nothing that reaches the row
         map_row<T, TEAM, false>(x, mk, d, V, nt, [](float, int) { return 0.f; });
     } else if (st.w != 0.f) {
         map_row<T, TEAM, MASK>(x, mk, d, V, nt, [&](float y, int i) {

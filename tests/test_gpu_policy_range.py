@@ -358,3 +358,21 @@ def test_rows_without_an_entry_get_no_gradient(n, V, dtype, rest):
             rows = p.distill_loss(leaf, t, ids, mask=mask, rest=rest, reduction="none")
             e, = torch.autograd.grad(rows.sum(), leaf)
             assert (rows[pad] == 0).all() and rows[n - 1] == 0 and (e[pad] == 0).all() and (e[n - 1] == 0).all()
+
+
+@pytest.mark.parametrize("n,V,dtype", FORMS)
+def test_actions_outside_get_no_gradient(n, V, dtype):
+    """Padding: an action outside 0..V-1 beside logits that are no numbers has log-probability 0 and no gradient."""
+    p = _policy()
+    x = _logits(n, V, DT[dtype])
+    a = _actions(n, V).clamp(0, V - 1)
+    a[n - 1] = -1
+    x[n - 1, V // 2:] = math.nan
+    x[n - 1, 0] = math.inf
+    for mask in (None, _mask("random", n, V)):
+        leaf = x.clone().requires_grad_(True)
+        r = p.action_logprobs(leaf, a.cuda(), mask=mask)
+        g, = torch.autograd.grad(r.logp.sum(), leaf, retain_graph=True)
+        assert r.logp[n - 1] == 0 and (g[n - 1] == 0).all() and g[:n - 1].isfinite().all()
+        g, = torch.autograd.grad(r.logp.sum() + r.entropy.sum(), leaf)
+        assert g[n - 1][slice(None) if mask is None else mask[n - 1]].isnan().all()
