@@ -172,6 +172,8 @@ def _distill_work(n, V, dtype, grad):
 
 
 def _work(nbytes, device):
+    if nbytes < 0:  # all else is checked by now
+        raise ValueError("more than 2^35 rows, or 2^60 logits")
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
