@@ -252,9 +252,9 @@ __device__ __forceinline__ double exp_f64(double t) {
 // ---- softmax statistics -------------------------------------------------------------------------
 // s = sum 2^u, w = sum u 2^u with u = x c - r and r a whole number near max x c: moving a sum to another r is exact
 // (a power of two), and x c - r is one rounding.  r follows the maximum lazily (u <= 8.5), and starts at -2^100 with
-// an empty sum.  From 2^24 on r is not next to max x c but f32's number next to it: off by up to 8 below 2^28, by more than
-// f32's exponents reach soon after.  A row whose r is at 2^28 or beyond (all its logits at a mask's fill, or one far
-// above the others) or that holds no number is done again by `Soft` below, with u = (x - m) c.
+// an empty sum.  From 2^24 on r is f32's number next to max x c and off by more than a half: by up to 8 below 2^28, by more
+// than f32's exponents reach soon after.  A row whose sum is out of proportion for that (its largest logit a mask's fill,
+// or one far above the others) or that holds no number is done again with u = (x - m) c (far_stat).
 // ENT: f32 sums with the entropy's; else s alone, in f64 beyond a thread's 16 or 32 terms (a KL is a difference of
 // near values: what s is off by comes to twenty times that of it).
 template <bool ENT>
@@ -318,48 +318,6 @@ __device__ __forceinline__ Sum<ENT> team_sum(Sum<ENT> a, Sum<ENT>* sh) {
     return a;
 }
 
-// (m, s, w): max, sum 2^u and sum u 2^u with u = (x - m) c, for the rows that Sum does not hold.  An empty set is
-// (LOWEST, 0, 0): a finite start, so that a -inf logit (u = -inf) and a row of the type's lowest value (u = 0)
-// both come out as they should.
-struct Soft {
-    float m, s, w;
-};
-__device__ __forceinline__ void soft_add(Soft& a, float x, float c) {
-    const float m = nmax(a.m, x);
-    const float d = nmax((a.m - m) * c, -1e30f), k = ex2(d);
-    const float u = (x - m) * c, e = ex2(u);
-    a.w = (k == 0.f ? 0.f : (a.w + d * a.s) * k) + e * nmax(u, -1000.f);
-    a.s = a.s * k + e;
-    a.m = m;
-}
-__device__ __forceinline__ Soft soft_join(Soft a, Soft b, float c) {
-    const float m = nmax(a.m, b.m);
-    const float da = nmax((a.m - m) * c, -1e30f), db = nmax((b.m - m) * c, -1e30f);
-    const float ka = ex2(da), kb = ex2(db);
-    Soft r;
-    r.m = m;
-    r.s = a.s * ka + b.s * kb;
-    r.w = (ka == 0.f ? 0.f : (a.w + da * a.s) * ka) + (kb == 0.f ? 0.f : (b.w + db * b.s) * kb);
-    return r;
-}
-__device__ __forceinline__ Soft wave_soft(Soft v, float c) {
-    for (int o = 32; o > 0; o >>= 1)
-        v = soft_join(v, Soft{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.w, o)}, c);
-    return v;
-}
-template <int TEAM>
-__device__ Soft team_soft(Soft v, float c, Soft* sh) {
-    v = wave_soft(v, c);
-    if constexpr (TEAM > 64) {
-        __syncthreads();  // sh may still be read as Sum
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = sh[0];
-        for (int i = 1; i < TEAM / 64; ++i) v = soft_join(v, sh[i], c);
-    }
-    return v;
-}
-
 // A row's statistics as the gradients use them: u = x c - ref, or (x - ref) c on a wide row; p = 2^(u - l2)
 template <bool ENT>
 struct Stat {
@@ -385,33 +343,35 @@ __device__ __forceinline__ float logp_of(float x, const Stat<true>& st, float l2
         p = LN2 * (__builtin_fmaf(x, c, -st.ref) - l2);
     return p > 0.f ? 0.f : p;
 }
-// is this sum a row's (some probability, all numbers, at a reference near its maximum: then s >= 2^-8, and s and w are
-// finite)?  An empty one is a row without a legal action, or a wide one.
+// is this sum one of up to V logits at a reference near their maximum?  Empty ones are not, nor what holds a NaN.  Off by
+// 16 and more, log2 s would cost the f32 results their last bits; a KL's logarithms are f64, and its gradient's factors
+// fit f32 up to 64 (a fill of -1e9 at temperature 1: 202 us as without, 326 done again, 8192 x 32768 bf16).
 template <bool ENT>
-__device__ __forceinline__ bool plain_sum(const Sum<ENT>& a) {
-    return a.s > 0.f && a.s < INFINITY && fabsf(a.r) < 268435456.f;
+__device__ __forceinline__ bool plain_sum(const Sum<ENT>& a, int V) {
+    constexpr float most = ENT ? 0x1p16f : 0x1p64f;
+    return a.s >= 1.f / most && a.s <= most * (float)V && fabsf(a.w) < INFINITY;
 }
 
-// The parts of a row that is split over blocks: (r, s, w or s in two words, kind).  A part that Sum does not hold
-// leaves s = 0 and its maximum's x c in place of r; where that is far below the other parts' r (a stretch of fills) the
-// part counts for nothing, else the row is done again.
-constexpr float PART_SUM = 0.f, PART_FAR = 1.f, PART_AGAIN = 2.f;  // PART_AGAIN: some logit is no number
-__device__ __forceinline__ float part_kind(bool plain, float max) {
-    return plain || max == -INFINITY ? PART_SUM : fabsf(max) < INFINITY ? PART_FAR : PART_AGAIN;
+// a and p of disjoint parts of a row -> a of both, at the larger reference.  A part without probability counts for
+// nothing, one that holds a NaN makes the sum one.
+template <bool ENT>
+__device__ __forceinline__ void stat_add(Stat<ENT>& a, Stat<ENT> p, float c) {
+    if (p.s == 0) return;
+    if (a.s == 0) {
+        a = p;
+        return;
+    }
+    const double d = place(p.ref, p.wide, c) - place(a.ref, a.wide, c);
+    if (d > 0.0) {
+        const Stat<ENT> t = a;
+        a = p;
+        p = t;
+    }
+    const float t = -fabsf((float)d);
+    const float k = a.wide || p.wide ? ex2(t) : __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(t, -4096.f));  // whole: exact
+    a.s += p.s * k;
+    if constexpr (ENT) a.w += k == 0.f ? 0.f : (p.w + t * p.s) * k;
 }
-struct FarParts {
-    float top = -INFINITY;
-    bool any = false, again = false;
-    __device__ __forceinline__ void add(float4 p) {
-        any = true;
-        again |= p.w == PART_AGAIN;
-        top = fmaxf(top, p.x * (p.x < 0.f ? 1.f - 0x1p-22f : 1.f + 0x1p-22f));  // x c is rounded, and so may r be
-    }
-    template <bool ENT>
-    __device__ __forceinline__ bool redo(const Sum<ENT>& a) const {
-        return any && (again || !(a.s > 0 && top < a.r - 300.f));
-    }
-};
 
 // order of the alternatives: larger logit first (NaN before all), then the lower index.  0: not an alternative.
 __device__ __forceinline__ unsigned long long order_key(float x, unsigned idx) {
@@ -527,15 +487,6 @@ __device__ __forceinline__ void row_pass(const T* x, const uint8_t* mk, int V, f
         row_pass<T, TEAM, MASK, ENT, TOP, false>(x, mk, V, c, a, mx, best, gmax, edit);
 }
 
-// the row again, an element at a time, for what Sum does not hold
-template <class T, int TEAM, class Skip>
-__device__ Soft soft_pass(const T* x, const uint8_t* mk, int V, float c, Soft* sh, Skip skip) {
-    Soft v{LOWEST, 0.f, 0.f};
-    for (int i = team_tid<TEAM>(); i < V; i += TEAM)
-        if ((!mk || mk[i]) && !skip(i)) soft_add(v, (float)x[i], c);
-    return team_soft<TEAM>(v, c, sh);
-}
-
 template <int TEAM>
 __device__ __forceinline__ float team_max(float x, float* sh) {
     x = wave_max(x);
@@ -553,19 +504,66 @@ __device__ __forceinline__ float team_max(float x, float* sh) {
 template <bool ENT>
 union Shared {  // one reduction at a time
     Sum<ENT> sum[16];
-    Soft soft[16];
+    Stat<ENT> stat[16];
     float f[16];
 };
 
-// a row's statistics from its pass: as they are, or by the element-wise pass; an empty row has s = 0
-template <class T, int TEAM, bool ENT, class Skip>
-__device__ __forceinline__ Stat<ENT> row_stat(Sum<ENT> a, float mx, const T* x, const uint8_t* mk, int V, float c,
-                                              Shared<ENT>& sh, Skip skip) {
+// what Sum does not hold, from the logits' maximum m: a pass more.  An infinite m or a NaN makes s a NaN.
+template <class T, int TEAM, bool ENT, class Edit>
+__device__ __forceinline__ Stat<ENT> far_stat(float m, const T* x, const uint8_t* mk, int V, float c, Shared<ENT>& sh,
+                                              const Edit& edit) {
+    constexpr int N = VN<T>;
+    const int tid = team_tid<TEAM>(), nvec = V / N;
+    Sum<ENT> a{0.f, 0, 0.f};
+    auto add = [&](float y) {
+        const float u = (y - m) * c, e = ex2(u);
+        a.s += e;
+        if constexpr (ENT) a.w = __builtin_fmaf(e, nmax(u, -1000.f), a.w);
+    };
+    for (int vi = tid; vi < nvec; vi += TEAM) {
+        float f[N];
+        unpack<T>(load16<false>(x + (long long)vi * N), f);
+        if (mk) apply_mask<T>(mk + vi * N, f);
+        edit(vi, f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) add(f[i]);
+    }
+    const int i = nvec * N + tid;
+    if (i < V && (!mk || mk[i]) && !edit.one(i)) add((float)x[i]);
     a = team_sum<TEAM, ENT>(a, sh.sum);
-    if (plain_sum(a)) return Stat<ENT>{a.r, a.s, a.w, false};
-    if (team_max<TEAM>(mx, sh.f) == -INFINITY) return Stat<ENT>{0.f, 0, 0.f, false};
-    const Soft v = soft_pass<T, TEAM>(x, mk, V, c, sh.soft, skip);
-    return Stat<ENT>{v.m, v.s, v.w, true};
+    return Stat<ENT>{m, a.s, a.w, true};
+}
+
+// the statistics of a row, or of a part of it, from its pass; without a legal action s = 0
+template <class T, int TEAM, bool ENT, class Edit>
+__device__ __forceinline__ Stat<ENT> row_stat(Sum<ENT> a, float mx, const T* x, const uint8_t* mk, int V, float c,
+                                              Shared<ENT>& sh, const Edit& edit) {
+    a = team_sum<TEAM, ENT>(a, sh.sum);
+    if (plain_sum(a, V)) return Stat<ENT>{a.r, a.s, a.w, false};
+    mx = team_max<TEAM>(mx, sh.f);
+    if (mx == -INFINITY) return Stat<ENT>{0.f, 0, 0.f, false};
+    return far_stat<T, TEAM, ENT>(mx, x, mk, V, c, sh, edit);
+}
+
+// the statistics of a row from those of its parts, of which each thread has joined some
+template <int TEAM, bool ENT>
+__device__ __forceinline__ Stat<ENT> team_join(Stat<ENT> v, float c, Shared<ENT>& sh) {
+    const bool wide = TEAM == 64 ? __ballot(v.wide) != 0 : __syncthreads_or(v.wide);
+    if (!wide) {
+        const Sum<ENT> a = team_sum<TEAM, ENT>(Sum<ENT>{v.s == 0 ? -FAR : v.ref, v.s, v.w}, sh.sum);
+        return Stat<ENT>{a.s == 0 ? 0.f : a.r, a.s, a.w, false};
+    }
+    for (int o = 32; o > 0; o >>= 1)
+        stat_add(v, Stat<ENT>{__shfl_xor(v.ref, o), __shfl_xor(v.s, o), __shfl_xor(v.w, o), (bool)__shfl_xor((int)v.wide, o)}, c);
+    if constexpr (TEAM > 64) {
+        if ((threadIdx.x & 63) == 0) sh.stat[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = sh.stat[0];
+        for (int i = 1; i < TEAM / 64; ++i) stat_add(v, sh.stat[i], c);
+        return v;
+    }
+    // the first lane's for all: at one place two lanes may hold references of either kind
+    return Stat<ENT>{lane_of(v.ref, 0), lane_of(v.s, 0), lane_of(v.w, 0), lane_of((unsigned)v.wide, 0) != 0};
 }
 
 // ---- the k largest of a row -----------------------------------------------------------------------
@@ -851,22 +849,13 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
     float mx = -INFINITY;
     Best best{-INFINITY, 0};
     row_pass<T, TEAM, MASK, true, TOP>(x, mk, V, R.c, a, mx, best, gmax, NoEdit{}, r < O.keep);
-    Stat<true> st;
+    const Stat<true> st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, NoEdit{});
+    const bool numbers = st.s == st.s;  // no NaN, no +inf: the alternatives by their bound
     float l2 = 0.f;
-    bool numbers;  // no NaN, no +inf: the alternatives by their bound
     if constexpr (PART) {
-        a = team_sum<TEAM, true>(a, sh.sum);
-        const bool plain = plain_sum(a);
-        const float all = plain ? 0.f : team_max<TEAM>(mx, sh.f), kind = part_kind(plain, all);
-        numbers = kind != PART_AGAIN;
-        if (tid == 0)
-            P.part[r * P.n + blockIdx.z] = plain                ? make_float4(a.r, a.s, a.w, kind)
-                                           : kind == PART_SUM ? make_float4(-FAR, 0.f, 0.f, kind)
-                                                                : make_float4(all * R.c, 0.f, 0.f, kind);
+        if (tid == 0) P.part[r * P.n + blockIdx.z] = make_float4(st.ref, st.s, st.w, st.wide);
     } else {
-        st = row_stat<T, TEAM, true>(a, mx, x, mk, V, R.c, sh, [](int) { return false; });
         l2 = lg2(st.s);
-        numbers = st.s == st.s;
         if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
     }
     if constexpr (TOP) {
@@ -885,7 +874,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void logprobs_rows_kernel(Rows R, L
     }
 }
 
-// the parts of a row joined
+// rows split over blocks: the parts' statistics and alternatives joined
 template <class T, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut O, Split P) {
     __shared__ Shared<true> sh;
@@ -896,19 +885,10 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
     const uint8_t* mk = mask_ptr(R, r);
     const int tid = threadIdx.x;
     const long long act = action_of(O, r);
-    Sum<true> a{-FAR, 0.f, 0.f};
-    FarParts far;
+    Stat<true> st{0.f, 0.f, 0.f, false};
     for (int i = tid; i < P.n; i += 256) {
         const float4 p = P.part[r * P.n + i];
-        if (p.w != PART_SUM) {
-            far.add(p);
-            continue;
-        }
-        const float m = fmaxf(a.r, p.x);
-        const Sum<true> b = move_sum(Sum<true>{p.x, p.y, p.z}, m);
-        a = move_sum(a, m);
-        a.s += b.s;
-        a.w += b.w;
+        stat_add(st, Stat<true>{p.x, p.y, p.z, p.w != 0.f}, R.c);
     }
     unsigned long long best = 0;
     const unsigned long long* keys = nullptr;
@@ -917,12 +897,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(Rows R, LogprobsOut 
         keys = P.keys + r * nk;
         for (int i = tid; i < nk; i += 256) best = best > keys[i] ? best : keys[i];
     }
-    a = team_sum<256, true>(a, sh.sum);
-    Stat<true> st{a.s > 0.f ? a.r : 0.f, a.s, a.w, false};
-    if (__syncthreads_or(far.redo(a))) {
-        const Soft v = soft_pass<T, 256>(x, mk, R.V, R.c, sh.soft, [](int) { return false; });
-        st = Stat<true>{v.m, v.s, v.w, true};
-    }
+    st = team_join<256, true>(st, R.c, sh);
     const float l2 = lg2(st.s);
     if (tid == 0) write_row<T>(R, O, r, st, l2, act, x, mk);
     if constexpr (TOP) {
@@ -1417,7 +1392,7 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
         row_pass<T, TEAM, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
     }
     const Stat<false> v =
-        row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, [&](int i) { return skip.one(i); });
+        row_stat<T, TEAM, false>(a, mx, x, mk, V, R.c, sh, skip);
     if (tid < 64) {
         RowSums both;
         const Row o = row_coefficients(R, Te, E, h, v, repeats, &both);
@@ -1476,9 +1451,9 @@ void distill_rows_kernel(Rows R, Teacher Te, DistillOut O) {
 }
 
 // a part of a row of few rows: its statistics outside the entries
-__device__ __forceinline__ Sum<false> part_sum(float4 p) {
-    const unsigned long long w = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.y);
-    return Sum<false>{p.x, __longlong_as_double((long long)w), 0.f};
+__device__ __forceinline__ Stat<false> part_stat(float4 p) {
+    const unsigned long long s = ((unsigned long long)__float_as_uint(p.z) << 32) | __float_as_uint(p.y);
+    return Stat<false>{p.x, __longlong_as_double((long long)s), 0.f, p.w != 0.f};
 }
 template <class T, bool MASK>
 __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, DistillOut O, Split P) {
@@ -1509,13 +1484,11 @@ __global__ __launch_bounds__(256) void distill_part_kernel(Rows R, Teacher Te, D
     Best none{-INFINITY, 0};
     const SkipBits<T> skip{bits, Te.rest != 0};
     row_pass<T, 256, MASK, false, false>(x, mk, V, R.c, a, mx, none, nullptr, skip, r < O.keep);
-    a = team_sum<256, false>(a, sh.sum);
-    const bool plain = plain_sum(a);
-    const float all = plain ? 0.f : team_max<256>(mx, sh.f), kind = part_kind(plain, all);
+    const Stat<false> st = row_stat<T, 256, false>(a, mx, x, mk, V, R.c, sh, skip);
     if (tid == 0) {
-        const unsigned long long w = (unsigned long long)__double_as_longlong(plain ? a.s : 0.0);
-        P.part[r * P.n + blockIdx.z] = make_float4(plain ? a.r : kind == PART_SUM ? -FAR : all * R.c,
-                                                   __uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)), kind);
+        const unsigned long long s = (unsigned long long)__double_as_longlong(st.s);
+        P.part[r * P.n + blockIdx.z] =
+            make_float4(st.ref, __uint_as_float((unsigned)s), __uint_as_float((unsigned)(s >> 32)), st.wide);
     }
 }
 
@@ -1528,7 +1501,6 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     __shared__ Shared<false> sh;
     __shared__ Entries Es[TEAMS];
     __shared__ Row row;
-    __shared__ Stat<false> joined;
     // from parts: few rows, or long ones whose many coefficients a block should not work out for little of it
     const Part at = JOIN ? Part{R.rows - 1 - team_row<TEAM>(), (int)blockIdx.z * len} : part_of<TEAM>(R, len);
     const long long r = at.r;
@@ -1539,7 +1511,7 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     Entries& E = Es[team_in_block<TEAM>()];
     EntryHead h;
     bool repeats = false;
-    float4 part{-FAR, 0.f, 0.f, PART_SUM};  // ahead of the entries: their loads wait for each other
+    float4 part{0.f, 0.f, 0.f, 0.f};  // ahead of the entries: their loads wait for each other
     if constexpr (JOIN)
         if (tid < P.n) part = P.part[r * P.n + tid];
     if (tid < 64) {
@@ -1550,34 +1522,9 @@ __global__ __launch_bounds__(block_of<TEAM>) void distill_bwd_kernel(Rows R, Tea
     RowSums sums;
     if constexpr (JOIN) {
         if (tid < 64) {
-            Sum<false> a{-FAR, 0.0, 0.f};
-            FarParts far;
-            auto join = [&](float4 p) {
-                if (p.w != PART_SUM) return far.add(p);
-                const float m = fmaxf(a.r, p.x);
-                const Sum<false> b = move_sum(part_sum(p), m);
-                a = move_sum(a, m);
-                a.s += b.s;
-            };
-            join(part);
-            for (int i = tid + 64; i < P.n; i += 64) join(P.part[r * P.n + i]);
-            a = team_sum<64, false>(a, nullptr);
-            const bool again = __ballot(far.redo(a)) != 0;
-            if (tid == 0) joined = Stat<false>{a.s > 0.0 ? a.r : 0.f, a.s, 0.f, again};
-        }
-        __syncthreads();
-        Stat<false> v = joined;
-        if (v.wide) {
-            const bool rest = Te.rest;
-            const int k = Te.k;
-            const Soft s = soft_pass<T, TEAM>(x, mk, R.V, R.c, sh.soft, [&](int i) {
-                for (int j = 0; rest && j < k; ++j)
-                    if (E.id[j] == i) return true;
-                return false;
-            });
-            v = Stat<false>{s.m, s.s, 0.f, true};
-        }
-        if (tid < 64) {
+            Stat<false> v = part_stat(part);
+            for (int i = tid + 64; i < P.n; i += 64) stat_add(v, part_stat(P.part[r * P.n + i]), R.c);
+            v = team_join<64, false>(v, R.c, sh);
             o = row_coefficients(R, Te, E, h, v, repeats, &sums);
             if (tid == 0) row = o;
         }
