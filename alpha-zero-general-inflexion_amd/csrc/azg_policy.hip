@@ -16,12 +16,12 @@
 //
 // All of it is bound by HBM from some thousand rows x columns on, by chains of dependent steps and the call below.
 // On an MI355X (a 1 GiB copy reaches 5.2 TB/s, reading alone 6.4):
-//   scores, 8192 x 32768 bf16, top 8             93 us   5.8 TB/s of reads
-//   scores and gradient, 4092 x 50001 bf16       76 + 132 us (the second from the caches in part)
-//   loss alone, 4096 x 65536 f16, 16 entries     86 us   6.3 TB/s of reads
-//   loss with gradient, 8192 x 32768 bf16, 32   202 us   5.3 TB/s read and written once
-//   loss, then gradient, 2048 x 100003 f32, 128 138 + 300 us, 5.5 TB/s over both
-//   1 x 131072 bf16, top 20                      6.9 + 5.5 us (32 parts, joined)
+//   scores, 8192 x 32768 bf16, top 8             94 us   5.7 TB/s of reads
+//   scores and gradient, 4092 x 50001 bf16       78 + 132 us (the second from the caches in part)
+//   loss alone, 4096 x 65536 f16, 16 entries     86 us   6.2 TB/s of reads
+//   loss with gradient, 8192 x 32768 bf16, 32   203 us   5.3 TB/s read and written once
+//   loss, then gradient, 2048 x 100003 f32, 128 138 + 299 us, 5.5 TB/s over both
+//   1 x 131072 bf16, top 20                      7.1 + 5.7 us (32 parts, joined)
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -819,7 +819,7 @@ __device__ __forceinline__ void write_row(const Rows& R, const LogprobsOut& O, l
 
 // rows split over blocks
 struct Split {
-    float4* part;               // [rows][n]
+    float4* part;               // [rows][n]: a part's Stat (ref, s and w, or s in two words, wide)
     unsigned long long* keys;   // [rows][n][k], by rank, 0: none
     int n, len;                 // parts, elements in each but the last
 };

@@ -333,7 +333,7 @@ def distill_loss(logits, teacher_logp, teacher_ids, *, temperature=1.0, mask=Non
       rest=True   they are exp(teacher_logp), and what they leave of 1 is compared with all the mass that
                   the student gives to actions outside the entries (left out where it has none to give)
     reduction: "mean" (over all rows), "sum" (both 0-dim) or "none" ([...], f32).  A row without an entry or
-    without a legal action counts 0.  An entry at an action that the student cannot play (illegal, or a logit of
+    without a legal action counts 0 and gets no gradient, whatever its logits are.  An entry at an action that the student cannot play (illegal, or a logit of
     -inf) makes its row's loss +inf; its gradient is that of the others.  The teacher gets no gradient."""
     t = _check_logits("distill_loss", logits, temperature)
     if reduction not in ("mean", "sum", "none"):
@@ -351,8 +351,8 @@ def distill_loss(logits, teacher_logp, teacher_ids, *, temperature=1.0, mask=Non
 
 def distill_loss_grad(logits, teacher_logp, teacher_ids, *, temperature=1.0, mask=None, rest=False, weight=None):
     """(loss, gradient) of sum_r weight_r KL_r (distill_loss's rows) in one call: what a training step needs, with
-    one pass over the logits less than autograd.  weight: a number, or a tensor [...] of one per row; None: 1 / rows
-    (the mean).  The loss is 0-dim f32, the gradient has the logits' shape and type (a new contiguous tensor):
+    one pass over the logits less than autograd.  weight: a number, or a tensor [...] of one per row (any floating
+    type, taken as f32); None: 1 / rows (the mean).  The loss is 0-dim f32, the gradient has the logits' shape and type (a new contiguous tensor):
     logits.backward(gradient).  No autograd graph is built: in a training step captured in a HIP graph, or with the
     loss scaled from outside (weight), this is the form to take."""
     t = _check_logits("distill_loss_grad", logits, temperature)

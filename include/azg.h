@@ -482,9 +482,10 @@ int  azg_train_loss_bwd(const float* x3, int32_t ld3, const float* z4, int32_t l
  *   fewer than top: -inf / -1).  stats [rows][4] (16-B aligned, may be null) is what the backward needs.
  *   A row without a legal action: entropy 0, lse and logp -inf, ids -1.
  * azg_logprobs_bwd: dx [rows][vocab] (contiguous, logits' type) from the gradients of logp / entropy / lse
- *   (each may be null; element r at r * its stride, 0 repeats one value); 0 at illegal actions.
+ *   (each may be null; element r at r * its stride, 0 repeats one value); 0 at illegal actions, and in a row whose
+ *   action is outside [0, vocab) where g_entropy and g_lse are null.
  * azg_distill_fwd: row_loss [rows] = KL(teacher || student), 0 for a row without an entry or without a
- *   legal action; total (may be null) = scale sum_r weight_r row_loss_r (weight null: 1; a stride of 0
+ *   legal action, and so is its gradient; total (may be null) = scale sum_r weight_r row_loss_r (weight null: 1; a stride of 0
  *   repeats one value; f64, fixed order); dx (may be null) = the gradient of that sum.  stats [rows][8]
  *   (16-B aligned, may be null) is what azg_distill_bwd needs, which writes dx = the gradient of
  *   scale sum_r weight_r row_loss_r.
