@@ -5,7 +5,8 @@ import math
 import policy_oracle as po
 import pytest
 import torch
-from test_gpu_policy import DT, _actions, _check_distill, _check_logprobs, _full, _logits, _mask, _policy, _teacher
+from test_gpu_policy import (DT, _actions, _check_distill, _check_logprobs, _everything, _logits, _mask, _policy,
+                             _teacher)
 
 pytestmark = pytest.mark.gpu
 
@@ -376,3 +377,80 @@ def test_actions_outside_get_no_gradient(n, V, dtype):
         assert r.logp[n - 1] == 0 and (g[n - 1] == 0).all() and g[:n - 1].isfinite().all()
         g, = torch.autograd.grad(r.logp.sum() + r.entropy.sum(), leaf)
         assert g[n - 1][slice(None) if mask is None else mask[n - 1]].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_largest_vocabulary(dtype):
+    """2^29 actions, in thousands of parts: sums, alternatives, gradients up to the last element."""
+    p = _policy()
+    V = p.VOCAB_MAX
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty((1, V), dtype=DT[dtype], device="cuda")
+    for part in x[0].split(2 ** 27):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda"))
+    ids = torch.tensor([[0, V - 1, V // 2, 12345, V - 131073]], device="cuda")
+    x[0, ids[0]] = torch.tensor([20.0, 19.5, 19.0, 18.5, 18.0], device="cuda").to(x.dtype)
+    z = x[0].split(2 ** 27)
+    total = sum(q.double().sub(20).exp().sum() for q in z)
+    lse = 20 + total.log()
+    # 16 additions in a group, 2^20 / 4096 groups, 45 joining the threads and parts, exp and its argument: h each
+    tol = po.H * (16 + 256 + 45 + 40)
+    leaf = x.requires_grad_(True)
+    r = p.action_logprobs(leaf, ids[:, 1], top=5)
+    assert torch.equal(r.top_ids, ids)
+    assert abs(r.lse.item() - lse.item()) < tol + 3 * po.H * lse.item()
+    assert abs(r.logp.item() - (19.5 - lse.item())) < tol
+    none = p.action_logprobs(leaf.detach(), ids[:, 1])
+    assert abs(none.logp.item() - (19.5 - lse.item())) < tol
+    d, = torch.autograd.grad(r.logp, leaf)
+    t = torch.log(torch.tensor([[0.4, 0.3, 0.1, 0.1, 0.1]], device="cuda"))
+    loss, e = p.distill_loss_grad(leaf, t, ids, weight=1.0)
+    xe = torch.tensor([20.0, 19.5, 19.0, 18.5, 18.0], dtype=torch.float64, device="cuda")
+    want = (t.double().exp() * (t.double() - xe + lse)).sum()
+    assert abs(loss.item() - want.item()) < 40 * po.H + 2 * po.H * abs(want.item())
+    f, = torch.autograd.grad(p.distill_loss(leaf, t, ids), leaf)
+    eps = torch.finfo(x.dtype).eps / 2
+    q = t.double().exp() / t.double().exp().sum()
+    for i, part in enumerate(z):
+        lo = i * 2 ** 27
+        prob = (part.detach().double() - lse).exp()
+        # the exponential's argument is off by 4 h of its size in log2, 40 here
+        off = prob * (2 * tol + 200 * po.H + eps) + po.TINY[x.dtype]
+        for got, hot in ((-d, torch.tensor([[0.0, 1, 0, 0, 0]], dtype=torch.float64, device="cuda")), (e, q), (f, q)):
+            exact = prob.clone()
+            here = (ids[0] >= lo) & (ids[0] < lo + 2 ** 27)
+            exact[ids[0, here] - lo] -= hot[0, here]
+            most = off.clone()
+            most[ids[0, here] - lo] += hot[0, here] * (eps + 16 * po.H)
+            assert ((got[0, lo:lo + 2 ** 27].double() - exact).abs() <= most).all()
+
+
+@pytest.mark.parametrize("n,V,dtype", [(40, 343, "f32"), (2, 100003, "bf16"), (130, 20011, "f32")])
+def test_large_values_captured(n, V, dtype):
+    """The second pass within a graph, replayed with other inputs, with and without rows that take it."""
+    def inputs(seed):
+        x = _logits(n, V, DT[dtype], seed=seed)
+        t, ids = _teacher(x, 12, None, seed)
+        if seed % 2:
+            x[0] = -1e10
+            x[1, V // 3:] = 3e9
+            x[1, ids[1, :6]] = 7e11
+        return x, _actions(n, V, seed).cuda(), t.cuda(), ids.cuda()
+    bufs = [b.clone() for b in inputs(0)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _everything(*bufs, None)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _everything(*bufs, None)
+    for seed in (1, 2, 3, 4, 3):
+        new = inputs(seed)
+        for b, v in zip(bufs, new):
+            b.copy_(v)
+        graph.replay()
+        want = _everything(*new, None)
+        torch.cuda.synchronize()
+        for o, w in zip(out, want):
+            assert not o.isnan().any() and torch.equal(o, w), seed
